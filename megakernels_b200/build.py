@@ -14,8 +14,8 @@ import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB = os.path.join(HERE, os.environ.get("MK_B200_LIBNAME", "libmk_b200.so"))
-SOURCES = ["mk_api.cu", "mk_stage_api.cu", "mk_umma.cu", "mk_prefill.cu", "mk_prefill_08b.cu", "mk_serve.cu", "mk_sample.cu", "mk_attend.cu"]
-HEADERS = ["mk_common.h", "mk_device.cuh", "mk_decode.cuh", "mk_batch.cuh", "mk_stage.cuh", "mk_stage_ops.cuh", "mk_prefill.cuh", "mk_prefill_host.h", "mk_serve_host.h",
+SOURCES = ["mk_api.cu", "mk_stage_api.cu", "mk_umma.cu", "mk_prefill.cu", "mk_prefill_08b.cu", "mk_serve.cu", "mk_sample.cu", "mk_attend.cu", "mk_attend_rows.cu"]
+HEADERS = ["mk_common.h", "mk_device.cuh", "mk_decode.cuh", "mk_batch.cuh", "mk_stage.cuh", "mk_stage_ops.cuh", "mk_prefill.cuh", "mk_prefill_host.h", "mk_serve_host.h", "mk_attend.cuh",
            os.path.join("..", "..", "include", "mk_b200.h"), os.path.join("..", "..", "include", "mk_stage.h"),
            os.path.join("..", "..", "include", "mk_umma.h"), os.path.join("..", "..", "include", "mk_serve.h")]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "--fmad=false",

@@ -2,8 +2,8 @@
 
 Tolerances, in half steps h of the output's type (bf16 2^-9, fp16 2^-12 of a value's power of two, so at most 2^-8 and 2^-11 of the value).
 Heads: 32-bit arithmetic, so one rounding (h of the value) and 2^-20 of the head's largest value for the sums in between.  Attention: with E
-the largest |out| bound sum p |v| <= max |v|: one rounding h |out|, plus the probabilities' rounding.  16-bit caches: bf16 probabilities are two pieces (2^-16),
-fp16 ones one half (2^-11); scores are exact products in 32-bit sums whose error enters the exponent: 2^-20 max |score|.  4 bits: codes and queries are exact, probabilities and their
+the largest |out| bound sum p |v| <= max |v|: one rounding h |out|, plus the probabilities' rounding.  16-bit caches: bf16 probabilities are two pieces (2^-16) for
+few queries per request and one (2^-8 of each, so at most 2^-8 sum p |v|) for many, whose product takes both operands of one type; fp16 ones one half (2^-11); scores are exact products in 32-bit sums whose error enters the exponent: 2^-20 max |score|.  4 bits: codes and queries are exact, probabilities and their
 product with a scale are rounded to halves, lows too: 3 * 2^-11.  All of them times sum p |v| (for 4 bits sum p (|low| + 15 scale), at most 2 max |v| plus the low)."""
 
 import math
@@ -228,9 +228,9 @@ def case(kind, dtype, nq, nkv, dim, page, contexts, counts, window, sinks, seed=
     return cache, k, v, table.to(DEV), ints(contexts), starts, q
 
 
-def compare(got, want, cache, v, dtype):
+def compare(got, want, cache, v, dtype, many=False):
     big = float((v.abs().amax() if not cache.int4 else (cache.v_scales[..., 1].abs() + 15 * cache.v_scales[..., 0]).amax()))
-    slack = {"int4": 3 * 2.0 ** -11, torch.bfloat16: 2.0 ** -16, torch.float16: 2.0 ** -11}[cache.dtype] + 2.0 ** -14
+    slack = 2.0 ** -8 if many and cache.dtype == torch.bfloat16 else {"int4": 3 * 2.0 ** -11, torch.bfloat16: 2.0 ** -16, torch.float16: 2.0 ** -11}[cache.dtype] + 2.0 ** -14
     near(got, want, HALF[dtype], slack * big)
 
 
@@ -257,7 +257,7 @@ def test_attend_ragged_queries(kind, dtype, nq, nkv, dim):
     for window, sinks in ((0, 0), (33, 2), (100, 0)):
         cache, k, v, table, context, starts, q = case(kind, dtype, nq, nkv, dim, 32, contexts, counts, window, sinks, seed=window)
         got = paged.attend(q, cache, table, context, starts=starts, window=window, sinks=sinks, scale=0.11)
-        compare(got, R.attend(q, k, v, table, context, starts, 0.11, window, sinks), cache, v, dtype)
+        compare(got, R.attend(q, k, v, table, context, starts, 0.11, window, sinks), cache, v, dtype, many=True)
     paged.check()
 
 
@@ -321,7 +321,7 @@ def test_attend_sharp_scores():
     got = paged.attend(q, cache, table, context, starts=starts)
     want = R.attend(q, k, v, table, context, starts, 128 ** -0.5)
     # scores reach 30 * 2 * 40: their 32-bit error, 2^-20 of that, is the exponent's
-    near(got, want, HALF[torch.bfloat16], (2.0 ** -16 + 2.0 ** -20 * 3000) * float(v.abs().max()))
+    near(got, want, HALF[torch.bfloat16], (2.0 ** -8 + 2.0 ** -20 * 3000) * float(v.abs().max()))
 
 
 def test_attend_in_graphs_and_on_another_stream():
