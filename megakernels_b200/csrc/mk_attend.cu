@@ -530,6 +530,7 @@ static const char* bad_attend(const mk_attend_args* a) {
     if (a->q_heads < 1 || c.kv_heads > 65535 || a->q_heads % c.kv_heads || a->q_heads / c.kv_heads > MKV_MAX_GROUP_HEADS) return "query heads per KV head";
     if (!a->starts && a->tokens != a->requests) return "one query per request, or starts";
     if (a->window < 0 || a->sinks < 0 || a->max_new < 1) return "window, sinks or max_new";
+    if (!(a->scale > 0.f && a->scale < 1e30f)) return "scale (positive)";
     return nullptr;
 }
 

@@ -21,7 +21,7 @@
 namespace mkv {
 
 constexpr int R_ROWS = 128, R_KEYS = 128;
-enum { WA_EMPTY = 401, WA_FULL, WA_SCORES, WA_PROBS, WA_DONE };
+enum { WA_EMPTY = 401, WA_FULL, WA_SCORES, WA_PROBS, WA_DONE, WA_QUERIES };
 
 template <int HD, int KIND> struct RowsLayout {
     static constexpr int PRODUCERS = KIND == K_INT4 ? 8 : 4;          // warps
@@ -30,7 +30,7 @@ template <int HD, int KIND> struct RowsLayout {
     static constexpr int SLOT = R_KEYS * HD * 2 / CH, DEPTH = HD == 256 ? 4 : (HD == 128 ? 5 : 8), Q_BYTES = R_ROWS * HD * 2;
 };
 struct RowsShared {
-    uint64_t full[8], empty[8], scores[2], probs[2], done;
+    uint64_t full[8], empty[8], scores[2], probs[2], done, queries;
     uint32_t tmem;
     volatile int dead;
     int request, block;
@@ -83,7 +83,13 @@ __device__ __forceinline__ void tmem_ld32(uint32_t (&r)[32], uint32_t addr) {
                    "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
                  : "r"(addr));
 }
-__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// The registers of a load are its own until this wait: naming them here keeps every use behind it.
+__device__ __forceinline__ void tmem_wait_ld(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+                 :
+                 : "memory");
+}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
@@ -172,6 +178,7 @@ static __global__ void __launch_bounds__(RowsLayout<HD, KIND>::THREADS, 1) atten
         for (int i = 0; i < DEPTH; i++) mk::mbar_init(&S.full[i], L::PRODUCERS), mk::mbar_init(&S.empty[i], 1);
         for (int i = 0; i < 2; i++) mk::mbar_init(&S.scores[i], 1), mk::mbar_init(&S.probs[i], 4);
         mk::mbar_init(&S.done, 1);
+        mk::mbar_init(&S.queries, 4);
         mk::fence_barrier_init();
     }
     __syncthreads();
@@ -189,31 +196,6 @@ static __global__ void __launch_bounds__(RowsLayout<HD, KIND>::THREADS, 1) atten
     const int win_lo = A.window ? pos_lo - A.window + 1 : 0;
     auto key0_of = [&](int tile) { return (tile < tl.front ? tile : tl.from + tile - tl.front) * R_KEYS; };
 
-    // ---- the queries, a warp per row (rows behind the last repeat it)
-    for (int row = warp; row < R_ROWS; row += L::THREADS / 32) {
-        const int n = min(row, rows - 1), token = n / A.per, h = n - token * A.per;
-        const uint16_t* src = reinterpret_cast<const uint16_t*>(A.q) + (first + token0 + token) * A.q_tok + (long long)(head * A.per + h) * A.q_head;
-        uint4 x = make_uint4(0, 0, 0, 0);
-        const bool has = lane < HD / 8;
-        if (has) x = *reinterpret_cast<const uint4*>(src + lane * 8);
-        if constexpr (I4) {
-            float v[8], big = 0.f;
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const uint32_t w = (&x.x)[i >> 1];
-                v[i] = from16((uint16_t)(i & 1 ? w >> 16 : w), A.q_f16);
-                big = fmaxf(big, fabsf(v[i]));
-            }
-#pragma unroll
-            for (int d = 16; d; d >>= 1) big = fmaxf(big, __shfl_xor_sync(~0u, big, d));
-            const int e = exponent_of(big);
-            const float down = power(-e);
-            x = make_uint4(pack_half(v[0] * down, v[4] * down), pack_half(v[1] * down, v[5] * down), pack_half(v[2] * down, v[6] * down), pack_half(v[3] * down, v[7] * down));
-            if (lane == 0) S.q_exp[row] = e;
-        }
-        if (has) *reinterpret_cast<uint4*>(q_s + (lane >> 3) * (R_ROWS * 128) + row * 128 + (((lane & 7) ^ (row & 7)) << 4)) = x;
-    }
-    mk::fence_proxy_async();
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -223,15 +205,17 @@ static __global__ void __launch_bounds__(RowsLayout<HD, KIND>::THREADS, 1) atten
         // ================= producers: chunks in the order K0, K1 V0, K2 V1, ... (CH of each) ======================
         const int pw = warp - 4;
         uint32_t slot = 0, phase = 0;
-        int pending = -1;                                              // a slot whose copies are under way
+        int waiting = 0;                                               // chunks whose copies are under way: the last ones issued, two at most
         bool ok = true;
-        auto land = [&]() {
-            if (pending < 0) return;
-            cp_wait<0>();
+        auto arrived = [&](int back) {                                 // the chunk `back` before the next one has landed
             mk::fence_proxy_async();
             __syncwarp();
-            if (lane == 0) mk::mbar_arrive(&S.full[pending]);
-            pending = -1;
+            if (lane == 0) mk::mbar_arrive(&S.full[(slot + DEPTH - back) % DEPTH]);
+            waiting--;
+        };
+        auto land = [&]() {
+            cp_wait<0>();
+            while (waiting > 0) arrived(waiting);
         };
         auto room = [&](uint32_t s, uint32_t ph) {
             if (__all_sync(~0u, mk::mbar_try_wait(&S.empty[s], ph ^ 1u))) return true;
@@ -325,20 +309,30 @@ static __global__ void __launch_bounds__(RowsLayout<HD, KIND>::THREADS, 1) atten
 #pragma unroll
                     for (int c = 0; c < CH; c++) mk::mbar_arrive(&S.full[sl[c]]);
             } else {
+                // lane l < 8: where the tile's keys 16 l ... begin (they lie one after the other: a page holds whole runs of 16)
+                const uint8_t* run = (value ? A.v : A.k) + head * A.s_head + max(my_page, 0) * A.s_page + ((key0 + 16 * (lane & 7)) & ((1 << A.page_shift) - 1)) * A.s_pos;
+                const bool all_seen = key0 + R_KEYS - 1 <= pos_hi && (key0 >= win_lo || key0 + R_KEYS <= A.sinks) && __all_sync(~0u, my_page >= 0);
 #pragma unroll
                 for (int c = 0; c < CH; c++) {
-                    if (ok && !(ok = room(slot, phase))) break;
-                    uint8_t* dst = ring + slot * L::SLOT;
-                    const uint8_t* base = (value ? A.v : A.k) + head * A.s_head;
+                    if (!ok || !(ok = room(slot, phase))) break;
+                    const uint32_t dst = smem_u32(ring + slot * L::SLOT);
+                    // P pieces of 16 bytes of N rows from row_from; a warp copies 32 / P rows at a time
                     auto copy = [&](auto pieces_, auto rows_, int row_from, int byte_from) {
-                        constexpr int P = decltype(pieces_)::value, N = decltype(rows_)::value, AT_ONCE = 32 / P, SLAB = N * 128;
-#pragma unroll 4
-                        for (int i = 0; i < N / (4 * AT_ONCE); i++) {
-                            const int row = (i * 4 + pw) * AT_ONCE + lane / P, piece = lane % P, key = key0 + row_from + row;
-                            const int page = __shfl_sync(~0u, my_page, (row_from + row) >> 4);
-                            const bool live = page >= 0 && seen(key);
-                            const uint8_t* src = base + max(page, 0) * A.s_page + (key & ((1 << A.page_shift) - 1)) * A.s_pos + byte_from + piece * 16;
-                            cp16(smem_u32(dst) + (piece >> 3) * SLAB + row * 128 + (((piece & 7) ^ (row & 7)) << 4), src, live);
+                        constexpr int P = decltype(pieces_)::value, N = decltype(rows_)::value, AT_ONCE = 32 / P, SLAB = N * 128, STEP = 4 * AT_ONCE;
+                        const int piece = lane % P, row0 = pw * AT_ONCE + lane / P;
+                        const long long off = row0 * A.s_pos + byte_from + piece * 16;
+                        const uint32_t to = dst + (piece >> 3) * SLAB + row0 * 128;
+#pragma unroll
+                        for (int u = 0; u < N / 16; u++) {
+                            const int from = row_from / 16 + u;
+                            const uint8_t* src = reinterpret_cast<const uint8_t*>(__shfl_sync(~0u, (unsigned long long)run, from)) + off;
+                            const bool there = all_seen || __shfl_sync(~0u, my_page, from) >= 0;
+#pragma unroll
+                            for (int i = 0; i < 16 / STEP; i++) {
+                                const int row = i * STEP + row0;
+                                const bool live = all_seen || (there && seen(key0 + from * 16 + row));
+                                cp16(to + u * 2048 + i * STEP * 128 + (((piece & 7) ^ (row & 7)) << 4), src + i * STEP * A.s_pos, live);
+                            }
                         }
                     };
                     if constexpr (HD == 256) {
@@ -347,13 +341,11 @@ static __global__ void __launch_bounds__(RowsLayout<HD, KIND>::THREADS, 1) atten
                     } else if constexpr (HD == 128) copy(Const<16>{}, Const<128>{}, 0, 0);
                     else copy(Const<8>{}, Const<128>{}, 0, 0);
                     cp_commit();
-                    if (pending >= 0) {
-                        cp_wait<1>();
-                        mk::fence_proxy_async();
-                        __syncwarp();
-                        if (lane == 0) mk::mbar_arrive(&S.full[pending]);
+                    if (waiting == 2) {
+                        cp_wait<2>();
+                        arrived(2);
                     }
-                    pending = (int)slot;
+                    waiting++;
                     if (++slot == DEPTH) slot = 0, phase ^= 1u;
                 }
             }
@@ -394,7 +386,8 @@ static __global__ void __launch_bounds__(RowsLayout<HD, KIND>::THREADS, 1) atten
                 commit(&S.scores[tile & 1]);
                 return true;
             };
-            ok = tl.n == 0 || scores(0);
+            ok = rows_wait(S, A, &S.queries, 0, WA_QUERIES);
+            ok = ok && (tl.n == 0 || scores(0));
             for (int i = 0; i < tl.n && ok; i++) {
                 if (i + 1 < tl.n) {
                     // the accumulator still holds the probabilities of tile i - 1
@@ -418,9 +411,53 @@ static __global__ void __launch_bounds__(RowsLayout<HD, KIND>::THREADS, 1) atten
         }
         __syncwarp();
     } else {
-        // ================= softmax and output: thread = row ===========================================================
+        // ================= softmax and output: thread = row (rows behind the last repeat it) ==============================
         const int row = tid, n = min(row, rows - 1), token = n / A.per, h = n - token * A.per, pos = pos_lo + token;
         const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
+        {
+            // the queries: a warp's lanes copy its 32 rows one after the other
+            const uint16_t* own = reinterpret_cast<const uint16_t*>(A.q) + (first + token0 + token) * A.q_tok + (long long)(head * A.per + h) * A.q_head;
+            const bool has = lane < HD / 8;
+            auto from = [&](int i) { return reinterpret_cast<const uint16_t*>(__shfl_sync(~0u, (unsigned long long)own, i)) + lane * 8; };
+            auto place = [&](int i) { return q_s + (lane >> 3) * (R_ROWS * 128) + (warp * 32 + i) * 128 + (((lane & 7) ^ (i & 7)) << 4); };
+            if constexpr (I4) {
+#pragma unroll 1
+                for (int i0 = 0; i0 < 32; i0 += 8) {
+                    uint4 x[8];
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const uint16_t* p = from(i0 + i);
+                        x[i] = has ? *reinterpret_cast<const uint4*>(p) : make_uint4(0, 0, 0, 0);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        float v[8], big = 0.f;
+#pragma unroll
+                        for (int j = 0; j < 8; j++) {
+                            const uint32_t w = (&x[i].x)[j >> 1];
+                            v[j] = from16((uint16_t)(j & 1 ? w >> 16 : w), A.q_f16);
+                            big = fmaxf(big, fabsf(v[j]));
+                        }
+                        big = __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(big)));
+                        const int e = exponent_of(big);
+                        const float down = power(-e);
+                        if (lane == 0) S.q_exp[warp * 32 + i0 + i] = e;
+                        if (has) *reinterpret_cast<uint4*>(place(i0 + i)) = make_uint4(pack_half(v[0] * down, v[4] * down), pack_half(v[1] * down, v[5] * down), pack_half(v[2] * down, v[6] * down), pack_half(v[3] * down, v[7] * down));
+                    }
+                }
+            } else {
+#pragma unroll 8
+                for (int i = 0; i < 32; i++) {
+                    const uint16_t* p = from(i);
+                    if (has) cp16(smem_u32(place(i)), p, true);
+                }
+                cp_commit();
+                cp_wait<0>();
+            }
+            mk::fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mk::mbar_arrive(&S.queries);
+        }
         float ref = -INFINITY, sum = 0.f;
         const float scale = A.scale_log2 * (I4 ? power(S.q_exp[row]) : 1.f);
         bool ok = true;
@@ -433,47 +470,42 @@ static __global__ void __launch_bounds__(RowsLayout<HD, KIND>::THREADS, 1) atten
             const int key0 = key0_of(i);
             const uint32_t at = lanes + (i & 1) * 128, valid = *(volatile uint32_t*)&S.valid[i & 7];
             const bool whole = valid == 0xFFu && key0 + R_KEYS - 1 <= pos_lo && (!A.window || key0 > pos_hi - A.window || key0 + R_KEYS <= A.sinks);
-            auto hidden = [&](int c) {
-                const int key = key0 + c;
-                return key > pos || (A.window && key <= pos - A.window && key >= A.sinks) || !(valid >> (c >> 4) & 1);
-            };
-            // factors of a run of 16 keys: of its scores, and the exponent of its values
-            float f[2];
-            float ev[2] = {0.f, 0.f};
-            auto factors = [&](int c) {
+            // the keys this row sees, a bit each
+            uint32_t bits[4] = {~0u, ~0u, ~0u, ~0u};
+            if (!whole) {
+                auto below = [](int n, int w) { return n >= 32 * w + 32 ? ~0u : (n <= 32 * w ? 0u : (1u << (n - 32 * w)) - 1); };      // columns under n
 #pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    if constexpr (I4) {
-                        f[j] = scale * power(S.exps[i & 7][2 * c + j]);
-                        ev[j] = (float)S.exps[i & 7][8 + 2 * c + j];
-                    } else
-                        f[j] = scale;
-                }
-            };
-            uint32_t x[32];
-            float top = -INFINITY;
-#pragma unroll
-            for (int c = 0; c < 4; c++) {
-                tmem_ld32(x, at + c * 32);
-                factors(c);
-                tmem_wait_ld();
-                if (whole) {
-                    float a[2] = {-INFINITY, -INFINITY};
-                    if constexpr (I4) {
-#pragma unroll
-                        for (int j = 0; j < 32; j++) a[j >> 4] = fmaxf(a[j >> 4], __uint_as_float(x[j]) * f[j >> 4]);
-                        top = fmaxf(top, fmaxf(a[0] + ev[0], a[1] + ev[1]));
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 32; j++) a[j & 1] = fmaxf(a[j & 1], __uint_as_float(x[j]) * scale);
-                        top = fmaxf(top, fmaxf(a[0], a[1]));
-                    }
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 32; j++)
-                        if (!hidden(c * 32 + j)) top = fmaxf(top, fmaf(__uint_as_float(x[j]), f[j >> 4], ev[j >> 4]));
+                for (int w = 0; w < 4; w++) {
+                    bits[w] = below(pos - key0 + 1, w);
+                    if (A.window) bits[w] &= ~below(pos - A.window + 1 - key0, w) | below(A.sinks - key0, w);
+                    bits[w] &= (valid >> (2 * w) & 1 ? 0xFFFFu : 0u) | (valid >> (2 * w + 1) & 1 ? 0xFFFF0000u : 0u);
                 }
             }
+            // factors of a run of 16 keys: of its scores, and the exponent of its values
+            float f[8], ev[8];
+            if constexpr (I4) {
+#pragma unroll
+                for (int j = 0; j < 8; j++) f[j] = scale * power(S.exps[i & 7][j]), ev[j] = (float)S.exps[i & 7][8 + j];
+            }
+            uint32_t x[2][32];
+            float top = -INFINITY;
+            tmem_ld32(x[0], at);
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                tmem_wait_ld(x[c & 1]);
+                if (c < 3) tmem_ld32(x[(c + 1) & 1], at + (c + 1) * 32);
+                uint32_t (&y)[32] = x[c & 1];
+                if (!whole) {
+#pragma unroll
+                    for (int j = 0; j < 32; j++) y[j] = bits[c] >> j & 1 ? y[j] : 0xFF800000u;                   // -inf
+                }
+                float a[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int j = 0; j < 32; j++) a[j >> 4 | (j & 1) * 2] = fmaxf(a[j >> 4 | (j & 1) * 2], __uint_as_float(y[j]));
+                if constexpr (I4) top = fmaxf(top, fmaxf(fmaf(fmaxf(a[0], a[2]), f[2 * c], ev[2 * c]), fmaf(fmaxf(a[1], a[3]), f[2 * c + 1], ev[2 * c + 1])));
+                else top = fmaxf(top, fmaxf(fmaxf(a[0], a[2]), fmaxf(a[1], a[3])));
+            }
+            if constexpr (!I4) top *= scale;
             // the reference rises when a score exceeds it by 2^8
             if (__any_sync(~0u, top > ref + 8.f)) {
                 const float next = fmaxf(ref, top), turn = next == -INFINITY ? 1.f : exp2_fast(ref - next);
@@ -487,36 +519,41 @@ static __global__ void __launch_bounds__(RowsLayout<HD, KIND>::THREADS, 1) atten
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
                     for (int c = 0; c < HD / 32; c++) {
-                        tmem_ld32(x, lanes + T_O + c * 32);
-                        tmem_wait_ld();
+                        tmem_ld32(x[0], lanes + T_O + c * 32);
+                        tmem_wait_ld(x[0]);
 #pragma unroll
-                        for (int j = 0; j < 32; j++) x[j] = __float_as_uint(__uint_as_float(x[j]) * turn);
-                        tmem_st32(lanes + T_O + c * 32, x);
+                        for (int j = 0; j < 32; j++) x[0][j] = __float_as_uint(__uint_as_float(x[0][j]) * turn);
+                        tmem_st32(lanes + T_O + c * 32, x[0]);
                     }
                     tmem_wait_st();
                 }
             }
             const float base = ref == -INFINITY ? 0.f : ref;
+            tmem_ld32(x[0], at);
 #pragma unroll
             for (int c = 0; c < 4; c++) {
-                tmem_ld32(x, at + c * 32);
-                factors(c);
-                tmem_wait_ld();
-                float part[2] = {0.f, 0.f};
+                tmem_wait_ld(x[c & 1]);
+                if (c < 3) tmem_ld32(x[(c + 1) & 1], at + (c + 1) * 32);
+                uint32_t (&y)[32] = x[c & 1];
+                float part[4] = {0.f, 0.f, 0.f, 0.f};
                 uint32_t p[16];
-                const float b[2] = {ev[0] - base, ev[1] - base};
+#pragma unroll
+                for (int j = 0; j < 32; j++) {
+                    const float fj = I4 ? f[2 * c + (j >> 4)] : scale, bj = I4 ? ev[2 * c + (j >> 4)] - base : -base;
+                    y[j] = __float_as_uint(exp2_fast(fmaf(__uint_as_float(y[j]), fj, bj)));
+                }
+                if (!whole) {
+#pragma unroll
+                    for (int j = 0; j < 32; j++) y[j] = bits[c] >> j & 1 ? y[j] : 0u;
+                }
 #pragma unroll
                 for (int j = 0; j < 32; j += 2) {
-                    float u = exp2_fast(fmaf(__uint_as_float(x[j]), f[j >> 4], b[j >> 4])), v = exp2_fast(fmaf(__uint_as_float(x[j + 1]), f[j >> 4], b[j >> 4]));
-                    if (!whole) {
-                        if (hidden(c * 32 + j)) u = 0.f;
-                        if (hidden(c * 32 + j + 1)) v = 0.f;
-                    }
-                    part[j >> 4] += u + v;
+                    const float u = __uint_as_float(y[j]), v = __uint_as_float(y[j + 1]);
+                    part[j >> 4] += u, part[2 + (j >> 4)] += v;
                     p[j / 2] = BF ? pack_bf(u, v) : pack_half(u, v);
                 }
-                if constexpr (I4) sum += part[0] * power(-S.exps[i & 7][8 + 2 * c]) + part[1] * power(-S.exps[i & 7][9 + 2 * c]);
-                else sum += part[0] + part[1];
+                if constexpr (I4) sum += (part[0] + part[2]) * power(-S.exps[i & 7][8 + 2 * c]) + (part[1] + part[3]) * power(-S.exps[i & 7][9 + 2 * c]);
+                else sum += (part[0] + part[2]) + (part[1] + part[3]);
                 tmem_st16(at + c * 16, p);
             }
             tmem_wait_st();
@@ -524,7 +561,8 @@ static __global__ void __launch_bounds__(RowsLayout<HD, KIND>::THREADS, 1) atten
             __syncwarp();
             if (lane == 0) mk::mbar_arrive(&S.probs[i & 1]);
         }
-        if (ok && tl.n > 0) ok = __all_sync(~0u, rows_wait(S, A, &S.done, (tl.n - 1) & 1, WA_DONE));
+        // (one after the other: a parity names a phase only among two)
+        for (int i = max(tl.n - 2, 0); i < tl.n && ok; i++) ok = __all_sync(~0u, rows_wait(S, A, &S.done, i & 1, WA_DONE));
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         if (ok) {
             const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
@@ -534,7 +572,7 @@ static __global__ void __launch_bounds__(RowsLayout<HD, KIND>::THREADS, 1) atten
                 uint32_t x[32];
                 if (tl.n > 0) {
                     tmem_ld32(x, lanes + T_O + c * 32);
-                    tmem_wait_ld();
+                    tmem_wait_ld(x);
                 }
                 if (row < rows)
 #pragma unroll
