@@ -1,7 +1,7 @@
 // Attention of many queries per request over a paged cache (declarations and rule: include/mk_serve.h).
 //
 // attend_rows: a CTA owns 128 rows, the (token, query head) pairs of one KV head for 128 / (query heads per KV head) tokens, and passes
-// over the keys they see in tiles of 128.  Warps 0-3: one row per thread, softmax and output; warps 4 on: producers, which bring keys and values into a ring
+// over the keys they see in tiles of 128.  Warps 0-7: two threads a row, softmax and output; warps 4 on: producers, which bring keys and values into a ring
 // of shared memory in the tensor core's swizzled order; the last warp's lane issues the products:
 //   S = Q K^T    Q and K from shared memory (both K-major), 128 x 128 scores into one of two accumulators in tensor memory;
 //   O += P V     P from tensor memory, where the row's thread put it over its scores, V from shared memory as it lies (MN-major),
@@ -10,31 +10,35 @@
 // by 2^8 (in tensor memory, by the row's thread, behind the product before).
 //   Tiles of 128 keys because a product of 128 x 64 would read its operands from shared memory slower than it multiplies; keys (by dims) and values
 // (by keys) of a head of 256 come in halves, so that four 32 KB slots beside the 64 KB of Q hold two products ahead.
-//   16 bits: cp.async straight into place, rows that nobody sees as zeros.  Probabilities are rounded to the operands' type, as the product takes both of one type
+//   16 bits: one warp's tiled TMA loads straight into place (a box is a page's rows, 64 dims).  Rows of values that no query of the block may see can hold anything, so the
+// warp writes zeros over them before it hands the tile on; keys need no such care, their scores are masked.  Probabilities are rounded to the operands' type, as the product takes both of one type
 // (bf16: half of the output's own rounding again).
-//   4 bits: eight warps turn codes into halves, one rounding (2^-11) each: the values of 16 keys times a power of two of their own, 2^-E, so
+//   4 bits: four warps turn codes into halves, one rounding (2^-11) each: the values of 16 keys times a power of two of their own, 2^-E, so
 // that any bf16 scale fits.  Keys' E scales the scores; values' E is added to the scores' exponent (sum of p v = sum of (p 2^E)(v 2^-E)) and taken out of the denominator.
 // Codes 0 .. 7 of a word come out in the order 0 4 1 5 2 6 3 7; queries are stored and outputs read in the same order.
+#include <cuda.h>
+
 #include "mk_attend.cuh"
 #include "mk_device.cuh"
 
 namespace mkv {
 
 constexpr int R_ROWS = 128, R_KEYS = 128;
-enum { WA_EMPTY = 401, WA_FULL, WA_SCORES, WA_PROBS, WA_DONE, WA_QUERIES };
+enum { WA_EMPTY = 401, WA_FULL, WA_SCORES, WA_PROBS, WA_DONE, WA_QUERIES, WA_LANDED };
 
 template <int HD, int KIND> struct RowsLayout {
-    static constexpr int PRODUCERS = KIND == K_INT4 ? 8 : 4;          // warps
-    static constexpr int THREADS = (4 + PRODUCERS + 1) * 32;
+    static constexpr int PRODUCERS = KIND == K_INT4 ? 4 : 3;          // warps
+    static constexpr int THREADS = (8 + PRODUCERS + 1) * 32;
     static constexpr int CH = HD == 256 ? 2 : 1;                      // chunks of a tile's keys, and of its values
     static constexpr int SLOT = R_KEYS * HD * 2 / CH, DEPTH = HD == 256 ? 4 : (HD == 128 ? 5 : 8), Q_BYTES = R_ROWS * HD * 2;
 };
 struct RowsShared {
-    uint64_t full[8], empty[8], scores[2], probs[2], done, queries;
+    uint64_t full[8], empty[8], scores[2], probs[2], done, queries, landed[3];
     uint32_t tmem;
     volatile int dead;
     int request, block;
-    int warp_sums[16];
+    int warp_sums[20];
+    float tops[2][2][R_ROWS];            // a row's largest score of either half of a tile, by turns; at the end the sums
     int q_exp[R_ROWS];                   // 4 bits: the queries' powers of two
     int exps[8][16];                     // of a tile (mod 8: the ring holds five ahead at most): E of its eight runs of 16 keys, and of values
     uint32_t valid[8];                   // of a tile (mod 8): which runs lie in pages of the cache
@@ -130,11 +134,22 @@ __device__ __forceinline__ Tiles tiles_of(const AttendArgs& A, int lo, int hi) {
     return t;
 }
 
+// How the tensor maps of a 16-bit cache see it: dims (d, positions of a page and KV heads in the order of their strides, pages), boxes of 64 d and `box` positions.
+struct Maps {
+    CUtensorMap k, v, q;                 // q: (d, query heads, tokens), boxes of 64 d, a KV head's query heads and a block's tokens
+    int box, heads_inside;               // heads_inside: the KV head is the second dim, the position the third
+};
+__device__ __forceinline__ void tile_load(uint32_t dst, const CUtensorMap* map, int d, int second, int third, int page, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst), "l"(map), "r"(d), "r"(second), "r"(third),
+                 "r"(page), "r"(smem_u32(bar))
+                 : "memory");
+}
+
 template <int HD, int KIND>
-static __global__ void __launch_bounds__(RowsLayout<HD, KIND>::THREADS, 1) attend_rows(const __grid_constant__ AttendArgs A) {
+static __global__ void __launch_bounds__(RowsLayout<HD, KIND>::THREADS, 1) attend_rows(const __grid_constant__ AttendArgs A, const __grid_constant__ Maps M) {
     using L = RowsLayout<HD, KIND>;
     constexpr bool I4 = KIND == K_INT4, BF = KIND == K_BF16;
-    constexpr int G = HD / 64, CH = L::CH, DEPTH = L::DEPTH, MMA_WARP = 4 + L::PRODUCERS;
+    constexpr int G = HD / 64, CH = L::CH, DEPTH = L::DEPTH, MMA_WARP = 8 + L::PRODUCERS;
     constexpr uint32_t T_O = 256;                                      // tensor memory: scores 0-127, 128-255, outputs behind
     extern __shared__ __align__(16) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -175,10 +190,11 @@ static __global__ void __launch_bounds__(RowsLayout<HD, KIND>::THREADS, 1) atten
             }
     }
     if (tid == 32) {
-        for (int i = 0; i < DEPTH; i++) mk::mbar_init(&S.full[i], L::PRODUCERS), mk::mbar_init(&S.empty[i], 1);
-        for (int i = 0; i < 2; i++) mk::mbar_init(&S.scores[i], 1), mk::mbar_init(&S.probs[i], 4);
+        for (int i = 0; i < DEPTH; i++) mk::mbar_init(&S.full[i], I4 ? L::PRODUCERS : 1), mk::mbar_init(&S.empty[i], 1);
+        for (int i = 0; i < 2; i++) mk::mbar_init(&S.scores[i], 1), mk::mbar_init(&S.probs[i], 8);
         mk::mbar_init(&S.done, 1);
-        mk::mbar_init(&S.queries, 4);
+        mk::mbar_init(&S.queries, I4 ? 8 : 1);
+        for (int i = 0; i < 3; i++) mk::mbar_init(&S.landed[i], 1);
         mk::fence_barrier_init();
     }
     __syncthreads();
@@ -201,27 +217,12 @@ static __global__ void __launch_bounds__(RowsLayout<HD, KIND>::THREADS, 1) atten
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = S.tmem;
 
-    if (warp >= 4 && warp < MMA_WARP) {
+    if (warp >= 8 && warp < MMA_WARP) {
         // ================= producers: chunks in the order K0, K1 V0, K2 V1, ... (CH of each) ======================
-        const int pw = warp - 4;
-        uint32_t slot = 0, phase = 0;
-        int waiting = 0;                                               // chunks whose copies are under way: the last ones issued, two at most
+        const int pw = warp - 8;
+        uint32_t slot = 0, phase = 0, patches = 0;
         bool ok = true;
-        auto arrived = [&](int back) {                                 // the chunk `back` before the next one has landed
-            mk::fence_proxy_async();
-            __syncwarp();
-            if (lane == 0) mk::mbar_arrive(&S.full[(slot + DEPTH - back) % DEPTH]);
-            waiting--;
-        };
-        auto land = [&]() {
-            cp_wait<0>();
-            while (waiting > 0) arrived(waiting);
-        };
-        auto room = [&](uint32_t s, uint32_t ph) {
-            if (__all_sync(~0u, mk::mbar_try_wait(&S.empty[s], ph ^ 1u))) return true;
-            land();                                                    // nobody is kept waiting for what has arrived
-            return __all_sync(~0u, rows_wait(S, A, &S.empty[s], ph ^ 1u, WA_EMPTY)) != 0;
-        };
+        auto room = [&](uint32_t s, uint32_t ph) { return __all_sync(~0u, rows_wait(S, A, &S.empty[s], ph ^ 1u, WA_EMPTY)) != 0; };
         auto pages_of = [&](int key0) {
             // lane l < 8: the page of the tile's keys 16 l ..., -1 outside the cache
             const int key = key0 + 16 * (lane & 7), n = key >> A.page_shift;
@@ -229,129 +230,170 @@ static __global__ void __launch_bounds__(RowsLayout<HD, KIND>::THREADS, 1) atten
             return page >= 0 && page < A.pages ? page : -1;
         };
         auto seen = [&](int key) { return key <= pos_hi && (key >= win_lo || key < A.sinks); };
-        for (int step = 0; step <= 2 * tl.n - 1 && ok; step++) {
-            // step 0: K0; then K(i + 1), V(i) by turns; the last one V(n - 1)
-            const bool value = step == 2 * tl.n - 1 || (step > 0 && (step & 1) == 0);
-            const int tile = step == 0 ? 0 : (value ? (step == 2 * tl.n - 1 ? tl.n - 1 : step / 2 - 1) : (step + 1) / 2);
-            const int key0 = key0_of(tile), my_page = pages_of(key0);
-            if (!value && pw == 0) {
-                const uint32_t v = __ballot_sync(~0u, my_page >= 0) & 0xFFu;
-                if (lane == 0) S.valid[tile & 7] = v;
+        if constexpr (!I4) {
+            // the queries: a box of the block's tokens and the KV head's query heads is 128 rows or a few less (what the tensor holds behind
+            // the block's tokens fills rows that go nowhere)
+            if (pw == 0 && lane == 0) {
+                mk::mbar_expect_tx(&S.queries, (uint32_t)(per_tile * A.per * HD * 2));
+                for (int x = 0; x < G; x++)
+                    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_u32(q_s) + x * R_ROWS * 128), "l"(&M.q),
+                                 "r"(x * 64), "r"(head * A.per), "r"(first + token0), "r"(smem_u32(&S.queries))
+                                 : "memory");
             }
-            if constexpr (I4) {
-                // two threads a row: four runs of eight values of every group each
-                const int row = pw * 16 + (lane >> 1), half = lane & 1, page = __shfl_sync(~0u, my_page, pw), key = key0 + row;
+            __syncwarp();
+        }
+        // step 0: K0; then K(i + 1), V(i) by turns; the last one V(n - 1)
+        const int steps = 2 * tl.n;
+        auto is_value = [&](int step) { return step == steps - 1 || (step > 0 && (step & 1) == 0); };
+        auto tile_at = [&](int step) { return step == 0 ? 0 : (step == steps - 1 ? tl.n - 1 : ((step & 1) ? (step + 1) / 2 : step / 2 - 1)); };
+        auto tell_valid = [&](int tile, int my_page) {
+            const uint32_t v = __ballot_sync(~0u, my_page >= 0) & 0xFFu;
+            if (lane == 0) S.valid[tile & 7] = v;
+        };
+        if constexpr (I4) {
+            // Half a step at a time, 64 rows, two threads a row (four runs of eight values of every group each).  The codes of the next two halves
+            // are on their way while this one's are turned into halves, and the pages of the tile behind.
+            const int half = lane & 1;
+            int page_v = -1, page_k = tl.n ? pages_of(key0_of(0)) : -1, page_next = tl.n > 1 ? pages_of(key0_of(1)) : -1;      // of V(i), K(i + 1) and K(i + 2)
+            struct Raw {
+                uint32_t w[4 * G], m[G], of_values[G];
+            };
+            auto get = [&](int part, Raw& x) {
+                const int step = part >> 1, tile = tile_at(step), run = (part & 1) * 4 + pw, key = key0_of(tile) + run * 16 + (lane >> 1);
+                const bool value = is_value(step);
+                if (!value && !(part & 1) && step > 0) {                // on to the next tile's keys
+                    page_v = page_k, page_k = page_next;
+                    page_next = tile + 1 < tl.n ? pages_of(key0_of(tile + 1)) : -1;
+                }
+                const int my_page = value && step != steps - 1 ? page_v : page_k;                      // (the last values are those of the last keys)
+                if (!value && pw == 0 && !(part & 1)) tell_valid(tile, my_page);
+                const int page = __shfl_sync(~0u, my_page, run);
                 const bool live = page >= 0 && seen(key);
                 const long long at = (((long long)max(page, 0) * A.nkv + head) << A.page_shift) + (key & ((1 << A.page_shift) - 1));
-                uint32_t mk_[G], mv_[G], w[4 * G];
-                auto load = [&](uint32_t (&m)[G], const uint8_t* base) {
+                const uint8_t* src = (value ? A.v : A.k) + at * (HD / 2) + half * (HD / 4);
+#pragma unroll
+                for (int j = 0; j < G; j++) *reinterpret_cast<uint4*>(x.w + 4 * j) = live ? __ldg(reinterpret_cast<const uint4*>(src) + j) : make_uint4(0, 0, 0, 0);
+                auto scales = [&](uint32_t (&to)[G], const uint8_t* base, bool wanted) {
                     const uint8_t* p = base + at * (G * 4);
-                    if constexpr (G == 4) *reinterpret_cast<uint4*>(m) = live ? __ldg(reinterpret_cast<const uint4*>(p)) : make_uint4(0, 0, 0, 0);
-                    else if constexpr (G == 2) *reinterpret_cast<uint2*>(m) = live ? __ldg(reinterpret_cast<const uint2*>(p)) : make_uint2(0, 0);
-                    else m[0] = live ? __ldg(reinterpret_cast<const uint32_t*>(p)) : 0u;
+                    if constexpr (G == 4) *reinterpret_cast<uint4*>(to) = wanted ? __ldg(reinterpret_cast<const uint4*>(p)) : make_uint4(0, 0, 0, 0);
+                    else if constexpr (G == 2) *reinterpret_cast<uint2*>(to) = wanted ? __ldg(reinterpret_cast<const uint2*>(p)) : make_uint2(0, 0);
+                    else to[0] = wanted ? __ldg(reinterpret_cast<const uint32_t*>(p)) : 0u;
                 };
-                {
-                    const uint8_t* p = (value ? A.v : A.k) + at * (HD / 2) + half * (HD / 4);
+                scales(x.m, value ? A.vs : A.ks, live);
+                scales(x.of_values, A.vs, live && !value);
+            };
+            auto warp_exp = [&](const uint32_t (&s)[G]) {
+                float big = 0.f;
 #pragma unroll
-                    for (int j = 0; j < G; j++) *reinterpret_cast<uint4*>(w + 4 * j) = live ? __ldg(reinterpret_cast<const uint4*>(p) + j) : make_uint4(0, 0, 0, 0);
+                for (int g = 0; g < G; g++) big = fmaxf(big, fmaxf(15.f * __uint_as_float(s[g] << 16), fabsf(__uint_as_float(s[g] & 0xFFFF0000u))));
+                return exponent_of(__uint_as_float(__reduce_max_sync(~0u, __float_as_uint(big))));
+            };
+            uint32_t sl[CH];
+            auto put = [&](int part, const Raw& x) {
+                const int step = part >> 1, p = part & 1;
+                const bool value = is_value(step);
+                const int e = warp_exp(x.m);
+                if (!value) {
+                    const int ev = warp_exp(x.of_values), tile = tile_at(step) & 7;
+                    if (lane == 0) S.exps[tile][p * 4 + pw] = e, S.exps[tile][8 + p * 4 + pw] = ev;
                 }
-                auto warp_exp = [&](const uint32_t (&m)[G]) {
-                    float big = 0.f;
+                if (p == 0) {
+                    uint32_t ph[CH];
 #pragma unroll
-                    for (int g = 0; g < G; g++) big = fmaxf(big, fmaxf(15.f * __uint_as_float(m[g] << 16), fabsf(__uint_as_float(m[g] & 0xFFFF0000u))));
+                    for (int c = 0; c < CH; c++) {
+                        sl[c] = slot, ph[c] = phase;
+                        if (++slot == DEPTH) slot = 0, phase ^= 1u;
+                    }
 #pragma unroll
-                    for (int d = 16; d; d >>= 1) big = fmaxf(big, __shfl_xor_sync(~0u, big, d));
-                    return exponent_of(big);
-                };
-                int e;
-                if (value) {
-                    load(mv_, A.vs);
-                    e = warp_exp(mv_);
-                } else {
-                    load(mk_, A.ks);
-                    load(mv_, A.vs);
-                    e = warp_exp(mk_);
-                    const int ev = warp_exp(mv_);
-                    if (lane == 0) S.exps[tile & 7][pw] = e, S.exps[tile & 7][8 + pw] = ev;
+                    for (int c = 0; c < CH; c++) ok = ok && room(sl[c], ph[c]);
+                    if (!ok) return;
                 }
                 const float down = power(-e);
-                uint32_t s2[G], l2[G];
+                const int slab = (value ? R_KEYS / CH : R_KEYS) * 128, row = (p * 4 + pw) * 16 + (lane >> 1), row_in = value && CH == 2 ? row & 63 : row;   // (values: a chunk is 64 keys, keys: 128 dims)
 #pragma unroll
                 for (int g = 0; g < G; g++) {
-                    const uint32_t m = value ? mv_[g] : mk_[g];
-                    const float s = __uint_as_float(m << 16) * down, l = __uint_as_float(m & 0xFFFF0000u) * down;
-                    s2[g] = pack_half(s, s), l2[g] = pack_half(l, l);
-                }
-                // both chunks' slots
-                uint32_t sl[CH], ph[CH];
+                    const float s1 = __uint_as_float(x.m[g] << 16) * down, l1 = __uint_as_float(x.m[g] & 0xFFFF0000u) * down;
+                    const uint32_t s2 = pack_half(s1, s1), l2 = pack_half(l1, l1);
+                    const uint32_t to = CH == 1 ? sl[0] : (value ? (p ? sl[CH - 1] : sl[0]) : sl[g >> 1 & (CH - 1)]);
+                    uint8_t* dst = ring + to * L::SLOT + (CH == 2 && !value ? g & 1 : g) * slab + row_in * 128;
 #pragma unroll
-                for (int c = 0; c < CH; c++) {
-                    sl[c] = slot, ph[c] = phase;
-                    if (++slot == DEPTH) slot = 0, phase ^= 1u;
-                }
-#pragma unroll
-                for (int c = 0; c < CH; c++) ok = ok && room(sl[c], ph[c]);
-                if (!ok) break;
-                const int mine = value && CH == 2 ? row >> 6 : 0, row_in = value && CH == 2 ? row & 63 : row;   // (values: a chunk is 64 keys, keys: 128 dims)
-                const int slab = (value ? R_KEYS / CH : R_KEYS) * 128;
-#pragma unroll
-                for (int j = 0; j < 4; j++)
-#pragma unroll
-                    for (int g = 0; g < G; g++) {
-                        const uint32_t x = w[j * G + g];
-                        const uint4 h = make_uint4(fma_half2(codes<0>(x), s2[g], l2[g]), fma_half2(codes<1>(x), s2[g], l2[g]), fma_half2(codes<2>(x), s2[g], l2[g]), fma_half2(codes<3>(x), s2[g], l2[g]));
-                        const int chunk = value ? mine : (CH == 2 ? g >> 1 : 0), slab_no = value ? g : (CH == 2 ? g & 1 : g);
-                        *reinterpret_cast<uint4*>(ring + sl[CH == 2 ? chunk : 0] * L::SLOT + slab_no * slab + row_in * 128 + (((half * 4 + j) ^ (row & 7)) << 4)) = h;
+                    for (int j = 0; j < 4; j++) {
+                        const uint32_t c = x.w[j * G + g];
+                        *reinterpret_cast<uint4*>(dst + (((half * 4 + j) ^ (row & 7)) << 4)) =
+                            make_uint4(fma_half2(codes<0>(c), s2, l2), fma_half2(codes<1>(c), s2, l2), fma_half2(codes<2>(c), s2, l2), fma_half2(codes<3>(c), s2, l2));
                     }
-                mk::fence_proxy_async();
+                }
+                if (p == 1) {
+                    mk::fence_proxy_async();
+                    __syncwarp();
+                    if (lane == 0)
+#pragma unroll
+                        for (int c = 0; c < CH; c++) mk::mbar_arrive(&S.full[sl[c]]);
+                }
+            };
+            Raw x, y, z;
+            const int parts = 2 * steps;
+            auto one = [&](int part, const Raw& now, Raw& far) {
+                if (part >= parts || !ok) return;
+                if (part + 2 < parts) get(part + 2, far);
+                put(part, now);
+            };
+            if (parts) get(0, x), get(1, y);
+            for (int part = 0; part < parts && ok; part += 3) {
+                one(part, x, z);
+                one(part + 1, y, x);
+                one(part + 2, z, y);
+            }
+        } else {
+            // the warps take chunks by turns: issuing one's loads takes as long as multiplying it
+            const int box_shift = 31 - __clz(M.box);
+            for (int q = pw; q < steps * CH && ok; q += L::PRODUCERS) {
+                const int step = q / CH, c = q % CH, tile = tile_at(step), key0 = key0_of(tile), my_page = pages_of(key0);
+                const bool value = is_value(step);
+                slot = q % DEPTH, phase = q / DEPTH & 1;
+                if (!value && c == 0) tell_valid(tile, my_page);
+                // keys that a query of the block, or of a later one, sees hold values; so do all sinks
+                const uint32_t pages = __ballot_sync(~0u, my_page >= 0);                                   // a bit per run of 16 keys (boxes are whole pages, or parts of one)
+                const bool clean = (pages & 0xFFu) == 0xFFu && key0 + R_KEYS <= context && (key0 >= win_lo || key0 + R_KEYS <= A.sinks);
+                uint8_t* dst = ring + slot * L::SLOT;
+                // keys: all 128, dims 128 c ...; values (of a head of 256): keys 64 c ..., all dims
+                const bool by_keys = value && CH == 2;
+                const int n = by_keys ? 64 : R_KEYS, from = by_keys ? 64 * c : 0, d0 = by_keys ? 0 : c * 128, slab_shift = HD == 64 ? 0 : (by_keys ? 2 : 1);
+                uint64_t* bar = value && !clean ? &S.landed[pw] : &S.full[slot];
+                const int x = lane & ((1 << slab_shift) - 1), row = (lane >> slab_shift) << box_shift, off = (key0 + from + row) & ((1 << A.page_shift) - 1);
+                const int page = __shfl_sync(~0u, my_page, (from + row) >> 4 & 7);
+                const bool mine = row < n && page >= 0;
+                const uint32_t loads = __popc(__ballot_sync(~0u, mine));
+                if (!(ok = room(slot, phase))) break;
+                if (lane == 0) {
+                    if (loads) mk::mbar_expect_tx(bar, loads * M.box * 128);
+                    else mk::mbar_arrive(bar);
+                }
                 __syncwarp();
-                if (lane == 0)
-#pragma unroll
-                    for (int c = 0; c < CH; c++) mk::mbar_arrive(&S.full[sl[c]]);
-            } else {
-                // lane l < 8: where the tile's keys 16 l ... begin (they lie one after the other: a page holds whole runs of 16)
-                const uint8_t* run = (value ? A.v : A.k) + head * A.s_head + max(my_page, 0) * A.s_page + ((key0 + 16 * (lane & 7)) & ((1 << A.page_shift) - 1)) * A.s_pos;
-                const bool all_seen = key0 + R_KEYS - 1 <= pos_hi && (key0 >= win_lo || key0 + R_KEYS <= A.sinks) && __all_sync(~0u, my_page >= 0);
-#pragma unroll
-                for (int c = 0; c < CH; c++) {
-                    if (!ok || !(ok = room(slot, phase))) break;
-                    const uint32_t dst = smem_u32(ring + slot * L::SLOT);
-                    // P pieces of 16 bytes of N rows from row_from; a warp copies 32 / P rows at a time
-                    auto copy = [&](auto pieces_, auto rows_, int row_from, int byte_from) {
-                        constexpr int P = decltype(pieces_)::value, N = decltype(rows_)::value, AT_ONCE = 32 / P, SLAB = N * 128, STEP = 4 * AT_ONCE;
-                        const int piece = lane % P, row0 = pw * AT_ONCE + lane / P;
-                        const long long off = row0 * A.s_pos + byte_from + piece * 16;
-                        const uint32_t to = dst + (piece >> 3) * SLAB + row0 * 128;
-#pragma unroll
-                        for (int u = 0; u < N / 16; u++) {
-                            const int from = row_from / 16 + u;
-                            const uint8_t* src = reinterpret_cast<const uint8_t*>(__shfl_sync(~0u, (unsigned long long)run, from)) + off;
-                            const bool there = all_seen || __shfl_sync(~0u, my_page, from) >= 0;
-#pragma unroll
-                            for (int i = 0; i < 16 / STEP; i++) {
-                                const int row = i * STEP + row0;
-                                const bool live = all_seen || (there && seen(key0 + from * 16 + row));
-                                cp16(to + u * 2048 + i * STEP * 128 + (((piece & 7) ^ (row & 7)) << 4), src + i * STEP * A.s_pos, live);
-                            }
-                        }
-                    };
-                    if constexpr (HD == 256) {
-                        if (value) copy(Const<32>{}, Const<64>{}, c * 64, 0);
-                        else copy(Const<16>{}, Const<128>{}, 0, c * 256);
-                    } else if constexpr (HD == 128) copy(Const<16>{}, Const<128>{}, 0, 0);
-                    else copy(Const<8>{}, Const<128>{}, 0, 0);
-                    cp_commit();
-                    if (waiting == 2) {
-                        cp_wait<2>();
-                        arrived(2);
+                if (mine)
+                    tile_load(smem_u32(dst) + x * n * 128 + row * 128, value ? &M.v : &M.k, d0 + x * 64, M.heads_inside ? head : off, M.heads_inside ? off : head, page, bar);
+                __syncwarp();
+                if (value && !clean) {
+                    if (!(ok = __all_sync(~0u, rows_wait(S, A, &S.landed[pw], patches & 1, WA_LANDED)) != 0)) break;
+                    patches++;
+                    // a lane per row; the pieces by turns, so that the lanes' stores spread over the banks
+                    for (int r0 = 0; r0 < n; r0 += 32) {
+                        const int line = r0 + lane;
+                        if (!(pages >> ((from + line) >> 4) & 1) || !seen(key0 + from + line))
+#pragma unroll 8
+                            for (int i = 0; i < 8 << slab_shift; i++) *reinterpret_cast<uint4*>(dst + (i >> 3) * n * 128 + line * 128 + ((i + lane & 7) << 4)) = make_uint4(0, 0, 0, 0);
                     }
-                    waiting++;
-                    if (++slot == DEPTH) slot = 0, phase ^= 1u;
+                    mk::fence_proxy_async();
+                    __syncwarp();
+                    if (lane == 0) mk::mbar_arrive(&S.full[slot]);
                 }
             }
         }
-        if (ok) land();
-        cp_wait<0>();
+        if (!I4 && S.dead) {
+            // loads under way still write shared memory: a bounded wait for them
+            const unsigned long long t0 = mk::globaltimer();
+            while (mk::globaltimer() - t0 < 1000000ull) {}
+        }
     } else if (warp == MMA_WARP) {
         // ================= the products ===============================================================================
         if (lane == 0) {
@@ -403,7 +445,7 @@ static __global__ void __launch_bounds__(RowsLayout<HD, KIND>::THREADS, 1) atten
 #pragma unroll
                     for (int x = 0; x < KEYS / 16; x++)
                         asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n"
-                                     ::"r"(tmem + T_O), "r"(tmem + (i & 1) * 128 + c * (KEYS / 2) + x * 8), "l"(db + x * 128), "r"(id_o), "r"((uint32_t)(i + c + x > 0)));
+                                     ::"r"(tmem + T_O), "r"(tmem + (i & 1) * 128 + (c * KEYS + x * 16) / 64 * 64 + (c * KEYS + x * 16) % 64 / 2), "l"(db + x * 128), "r"(id_o), "r"((uint32_t)(i + c + x > 0)));
                     release();
                 }
                 if (ok) commit(&S.done);
@@ -411,156 +453,144 @@ static __global__ void __launch_bounds__(RowsLayout<HD, KIND>::THREADS, 1) atten
         }
         __syncwarp();
     } else {
-        // ================= softmax and output: thread = row (rows behind the last repeat it) ==============================
-        const int row = tid, n = min(row, rows - 1), token = n / A.per, h = n - token * A.per, pos = pos_lo + token;
-        const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
-        {
-            // the queries: a warp's lanes copy its 32 rows one after the other
+        // ================= softmax and output: two threads a row, 64 keys (later half of the dims) each; rows behind the last repeat it ====
+        const int half = warp >> 2, row = tid & 127, n = min(row, rows - 1), token = n / A.per, h = n - token * A.per, pos = pos_lo + token;
+        const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+        if constexpr (I4) {
+            // the queries: a warp's lanes turn 16 of its rows into halves one after the other
             const uint16_t* own = reinterpret_cast<const uint16_t*>(A.q) + (first + token0 + token) * A.q_tok + (long long)(head * A.per + h) * A.q_head;
             const bool has = lane < HD / 8;
-            auto from = [&](int i) { return reinterpret_cast<const uint16_t*>(__shfl_sync(~0u, (unsigned long long)own, i)) + lane * 8; };
-            auto place = [&](int i) { return q_s + (lane >> 3) * (R_ROWS * 128) + (warp * 32 + i) * 128 + (((lane & 7) ^ (i & 7)) << 4); };
-            if constexpr (I4) {
-#pragma unroll 1
-                for (int i0 = 0; i0 < 32; i0 += 8) {
-                    uint4 x[8];
+            uint4 x[16];
 #pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        const uint16_t* p = from(i0 + i);
-                        x[i] = has ? *reinterpret_cast<const uint4*>(p) : make_uint4(0, 0, 0, 0);
-                    }
+            for (int i = 0; i < 16; i++) {
+                const uint16_t* p = reinterpret_cast<const uint16_t*>(__shfl_sync(~0u, (unsigned long long)own, half * 16 + i)) + lane * 8;
+                x[i] = has ? *reinterpret_cast<const uint4*>(p) : make_uint4(0, 0, 0, 0);
+            }
 #pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        float v[8], big = 0.f;
+            for (int i = 0; i < 16; i++) {
+                const int at = (warp & 3) * 32 + half * 16 + i;
+                float v[8], big = 0.f;
 #pragma unroll
-                        for (int j = 0; j < 8; j++) {
-                            const uint32_t w = (&x[i].x)[j >> 1];
-                            v[j] = from16((uint16_t)(j & 1 ? w >> 16 : w), A.q_f16);
-                            big = fmaxf(big, fabsf(v[j]));
-                        }
-                        big = __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(big)));
-                        const int e = exponent_of(big);
-                        const float down = power(-e);
-                        if (lane == 0) S.q_exp[warp * 32 + i0 + i] = e;
-                        if (has) *reinterpret_cast<uint4*>(place(i0 + i)) = make_uint4(pack_half(v[0] * down, v[4] * down), pack_half(v[1] * down, v[5] * down), pack_half(v[2] * down, v[6] * down), pack_half(v[3] * down, v[7] * down));
-                    }
+                for (int j = 0; j < 8; j++) {
+                    const uint32_t w = (&x[i].x)[j >> 1];
+                    v[j] = from16((uint16_t)(j & 1 ? w >> 16 : w), A.q_f16);
+                    big = fmaxf(big, fabsf(v[j]));
                 }
-            } else {
-#pragma unroll 8
-                for (int i = 0; i < 32; i++) {
-                    const uint16_t* p = from(i);
-                    if (has) cp16(smem_u32(place(i)), p, true);
-                }
-                cp_commit();
-                cp_wait<0>();
+                big = __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(big)));
+                const int e = exponent_of(big);
+                const float down = power(-e);
+                if (lane == 0) S.q_exp[at] = e;
+                if (has)
+                    *reinterpret_cast<uint4*>(q_s + (lane >> 3) * (R_ROWS * 128) + at * 128 + (((lane & 7) ^ (at & 7)) << 4)) =
+                        make_uint4(pack_half(v[0] * down, v[4] * down), pack_half(v[1] * down, v[5] * down), pack_half(v[2] * down, v[6] * down), pack_half(v[3] * down, v[7] * down));
             }
             mk::fence_proxy_async();
             __syncwarp();
             if (lane == 0) mk::mbar_arrive(&S.queries);
         }
+        // barrier of the eight warps; whether any of them has given up, the same answer for all
+        auto failed = [](bool mine) {
+            uint32_t any;
+            asm volatile("{\n .reg .pred p, q;\n setp.ne.u32 q, %1, 0;\n bar.red.or.pred p, 1, 256, q;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(any) : "r"((uint32_t)mine) : "memory");
+            return any != 0;
+        };
+        if constexpr (I4) failed(false);
         float ref = -INFINITY, sum = 0.f;
         const float scale = A.scale_log2 * (I4 ? power(S.q_exp[row]) : 1.f);
         bool ok = true;
         for (int i = 0; i < tl.n; i++) {
-            if (!__all_sync(~0u, rows_wait(S, A, &S.scores[i & 1], (i >> 1) & 1, WA_SCORES))) {
-                ok = false;
-                break;
-            }
+            ok = __all_sync(~0u, rows_wait(S, A, &S.scores[i & 1], (i >> 1) & 1, WA_SCORES)) && ok;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const int key0 = key0_of(i);
-            const uint32_t at = lanes + (i & 1) * 128, valid = *(volatile uint32_t*)&S.valid[i & 7];
+            const uint32_t at = lanes + (i & 1) * 128 + half * 64, valid = *(volatile uint32_t*)&S.valid[i & 7];
             const bool whole = valid == 0xFFu && key0 + R_KEYS - 1 <= pos_lo && (!A.window || key0 > pos_hi - A.window || key0 + R_KEYS <= A.sinks);
             // the keys this row sees, a bit each
-            uint32_t bits[4] = {~0u, ~0u, ~0u, ~0u};
+            uint32_t bits[2] = {~0u, ~0u};
             if (!whole) {
                 auto below = [](int n, int w) { return n >= 32 * w + 32 ? ~0u : (n <= 32 * w ? 0u : (1u << (n - 32 * w)) - 1); };      // columns under n
 #pragma unroll
-                for (int w = 0; w < 4; w++) {
-                    bits[w] = below(pos - key0 + 1, w);
-                    if (A.window) bits[w] &= ~below(pos - A.window + 1 - key0, w) | below(A.sinks - key0, w);
-                    bits[w] &= (valid >> (2 * w) & 1 ? 0xFFFFu : 0u) | (valid >> (2 * w + 1) & 1 ? 0xFFFF0000u : 0u);
+                for (int c = 0; c < 2; c++) {
+                    const int w = half * 2 + c;
+                    bits[c] = below(pos - key0 + 1, w);
+                    if (A.window) bits[c] &= ~below(pos - A.window + 1 - key0, w) | below(A.sinks - key0, w);
+                    bits[c] &= (valid >> (2 * w) & 1 ? 0xFFFFu : 0u) | (valid >> (2 * w + 1) & 1 ? 0xFFFF0000u : 0u);
                 }
             }
             // factors of a run of 16 keys: of its scores, and the exponent of its values
-            float f[8], ev[8];
+            float f[4], ev[4];
             if constexpr (I4) {
 #pragma unroll
-                for (int j = 0; j < 8; j++) f[j] = scale * power(S.exps[i & 7][j]), ev[j] = (float)S.exps[i & 7][8 + j];
+                for (int j = 0; j < 4; j++) f[j] = scale * power(S.exps[i & 7][half * 4 + j]), ev[j] = (float)S.exps[i & 7][8 + half * 4 + j];
             }
             uint32_t x[2][32];
             float top = -INFINITY;
             tmem_ld32(x[0], at);
+            tmem_ld32(x[1], at + 32);
+            tmem_wait_ld(x[0]);
+            tmem_wait_ld(x[1]);
+            if (!whole) {
 #pragma unroll
-            for (int c = 0; c < 4; c++) {
-                tmem_wait_ld(x[c & 1]);
-                if (c < 3) tmem_ld32(x[(c + 1) & 1], at + (c + 1) * 32);
-                uint32_t (&y)[32] = x[c & 1];
-                if (!whole) {
-#pragma unroll
-                    for (int j = 0; j < 32; j++) y[j] = bits[c] >> j & 1 ? y[j] : 0xFF800000u;                   // -inf
-                }
-                float a[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                for (int j = 0; j < 32; j++) a[j >> 4 | (j & 1) * 2] = fmaxf(a[j >> 4 | (j & 1) * 2], __uint_as_float(y[j]));
-                if constexpr (I4) top = fmaxf(top, fmaxf(fmaf(fmaxf(a[0], a[2]), f[2 * c], ev[2 * c]), fmaf(fmaxf(a[1], a[3]), f[2 * c + 1], ev[2 * c + 1])));
-                else top = fmaxf(top, fmaxf(fmaxf(a[0], a[2]), fmaxf(a[1], a[3])));
+                for (int j = 0; j < 64; j++) x[j >> 5][j & 31] = bits[j >> 5] >> (j & 31) & 1 ? x[j >> 5][j & 31] : 0xFF800000u;                   // -inf
             }
-            if constexpr (!I4) top *= scale;
+            float a[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int j = 0; j < 64; j++) a[j >> 4] = fmaxf(a[j >> 4], __uint_as_float(x[j >> 5][j & 31]));
+            if constexpr (I4) {
+#pragma unroll
+                for (int j = 0; j < 4; j++) top = fmaxf(top, fmaf(a[j], f[j], ev[j]));
+            } else
+                top = fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3])) * scale;
+            S.tops[i & 1][half][row] = top;
+            if (failed(!ok)) {                                         // (all eight warps leave together: they share this barrier)
+                ok = false;
+                break;
+            }
+            top = fmaxf(top, S.tops[i & 1][half ^ 1][row]);
             // the reference rises when a score exceeds it by 2^8
             if (__any_sync(~0u, top > ref + 8.f)) {
                 const float next = fmaxf(ref, top), turn = next == -INFINITY ? 1.f : exp2_fast(ref - next);
                 sum *= turn;
                 ref = next;
                 if (i > 0) {
-                    if (!__all_sync(~0u, rows_wait(S, A, &S.done, (i - 1) & 1, WA_DONE))) {
-                        ok = false;
-                        break;
-                    }
+                    ok = __all_sync(~0u, rows_wait(S, A, &S.done, (i - 1) & 1, WA_DONE)) && ok;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    uint32_t z[32];
 #pragma unroll 1
-                    for (int c = 0; c < HD / 32; c++) {
-                        tmem_ld32(x[0], lanes + T_O + c * 32);
-                        tmem_wait_ld(x[0]);
+                    for (int c = half * (HD / 64); c < (half + 1) * (HD / 64); c++) {
+                        tmem_ld32(z, lanes + T_O + c * 32);
+                        tmem_wait_ld(z);
 #pragma unroll
-                        for (int j = 0; j < 32; j++) x[0][j] = __float_as_uint(__uint_as_float(x[0][j]) * turn);
-                        tmem_st32(lanes + T_O + c * 32, x[0]);
+                        for (int j = 0; j < 32; j++) z[j] = __float_as_uint(__uint_as_float(z[j]) * turn);
+                        tmem_st32(lanes + T_O + c * 32, z);
                     }
                     tmem_wait_st();
                 }
             }
             const float base = ref == -INFINITY ? 0.f : ref;
-            tmem_ld32(x[0], at);
 #pragma unroll
-            for (int c = 0; c < 4; c++) {
-                tmem_wait_ld(x[c & 1]);
-                if (c < 3) tmem_ld32(x[(c + 1) & 1], at + (c + 1) * 32);
-                uint32_t (&y)[32] = x[c & 1];
+            for (int c = 0; c < 2; c++) {
                 float part[4] = {0.f, 0.f, 0.f, 0.f};
                 uint32_t p[16];
 #pragma unroll
-                for (int j = 0; j < 32; j++) {
-                    const float fj = I4 ? f[2 * c + (j >> 4)] : scale, bj = I4 ? ev[2 * c + (j >> 4)] - base : -base;
-                    y[j] = __float_as_uint(exp2_fast(fmaf(__uint_as_float(y[j]), fj, bj)));
-                }
-                if (!whole) {
-#pragma unroll
-                    for (int j = 0; j < 32; j++) y[j] = bits[c] >> j & 1 ? y[j] : 0u;
-                }
-#pragma unroll
                 for (int j = 0; j < 32; j += 2) {
-                    const float u = __uint_as_float(y[j]), v = __uint_as_float(y[j + 1]);
+                    const float fj = I4 ? f[2 * c + (j >> 4)] : scale, bj = I4 ? ev[2 * c + (j >> 4)] - base : -base;
+                    // (masked scores are -inf: their probability is 0)
+                    const float u = exp2_fast(fmaf(__uint_as_float(x[c][j]), fj, bj)), v = exp2_fast(fmaf(__uint_as_float(x[c][j + 1]), fj, bj));
                     part[j >> 4] += u, part[2 + (j >> 4)] += v;
                     p[j / 2] = BF ? pack_bf(u, v) : pack_half(u, v);
                 }
-                if constexpr (I4) sum += (part[0] + part[2]) * power(-S.exps[i & 7][8 + 2 * c]) + (part[1] + part[3]) * power(-S.exps[i & 7][9 + 2 * c]);
+                if constexpr (I4) sum += (part[0] + part[2]) * power(-S.exps[i & 7][8 + half * 4 + 2 * c]) + (part[1] + part[3]) * power(-S.exps[i & 7][9 + half * 4 + 2 * c]);
                 else sum += (part[0] + part[2]) + (part[1] + part[3]);
-                tmem_st16(at + c * 16, p);
+                tmem_st16(at + c * 16, p);                             // over scores that this thread has read
             }
             tmem_wait_st();
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
             if (lane == 0) mk::mbar_arrive(&S.probs[i & 1]);
         }
+        S.tops[tl.n & 1][half][row] = sum;
+        if (failed(!ok)) ok = false;                                   // nothing is written then
+        sum += S.tops[tl.n & 1][half ^ 1][row];
         // (one after the other: a parity names a phase only among two)
         for (int i = max(tl.n - 2, 0); i < tl.n && ok; i++) ok = __all_sync(~0u, rows_wait(S, A, &S.done, i & 1, WA_DONE));
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -568,7 +598,7 @@ static __global__ void __launch_bounds__(RowsLayout<HD, KIND>::THREADS, 1) atten
             const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
             uint16_t* dst = reinterpret_cast<uint16_t*>(A.out) + (first + token0 + token) * A.out_tok + (long long)(head * A.per + h) * A.out_head;
 #pragma unroll 1
-            for (int c = 0; c < HD / 32; c++) {
+            for (int c = half * (HD / 64); c < (half + 1) * (HD / 64); c++) {
                 uint32_t x[32];
                 if (tl.n > 0) {
                     tmem_ld32(x, lanes + T_O + c * 32);
@@ -604,6 +634,43 @@ static __global__ void __launch_bounds__(RowsLayout<HD, KIND>::THREADS, 1) atten
     }
 }
 
+typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+static EncodeTiled encode_tiled() {
+    static const EncodeTiled fn = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        return cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &found) == cudaSuccess && found == cudaDriverEntryPointSuccess ? reinterpret_cast<EncodeTiled>(p) : nullptr;
+    }();
+    return fn;
+}
+
+static int make_maps(const AttendArgs& A, int head_dim, bool f16, Maps* M) {
+    memset(M, 0, sizeof *M);
+    const EncodeTiled encode = encode_tiled();
+    if (!encode) return vfail(MK_ERR_CUDA, "mk_attend: the driver has no cuTensorMapEncodeTiled");
+    const int page = 1 << A.page_shift, most = head_dim == 256 ? 64 : R_KEYS;
+    M->box = page < most ? page : most;
+    // (the stride of an extent of one says nothing, and may be 0)
+    const long long s_head = A.nkv > 1 ? A.s_head : A.s_pos << A.page_shift, s_page = A.pages > 1 ? A.s_page : (A.s_pos << A.page_shift) * A.nkv;
+    M->heads_inside = s_head < A.s_pos;
+    const cuuint64_t size[4] = {(cuuint64_t)head_dim, (cuuint64_t)(M->heads_inside ? A.nkv : page), (cuuint64_t)(M->heads_inside ? page : A.nkv), (cuuint64_t)A.pages};
+    const cuuint64_t stride[3] = {(cuuint64_t)(M->heads_inside ? s_head : A.s_pos), (cuuint64_t)(M->heads_inside ? A.s_pos : s_head), (cuuint64_t)s_page};
+    const cuuint32_t box[4] = {64, (cuuint32_t)(M->heads_inside ? 1 : M->box), (cuuint32_t)(M->heads_inside ? M->box : 1), 1}, step[4] = {1, 1, 1, 1};
+    for (int i = 0; i < 2; i++) {
+        const CUresult rc = encode(i ? &M->v : &M->k, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<uint8_t*>(i ? A.v : A.k), size, stride, box, step,
+                                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+        if (rc != CUDA_SUCCESS) return vfail(MK_ERR_CUDA, "mk_attend: no tensor map for strides %lld, %lld, %lld bytes (error %d)", A.s_pos, A.s_head, A.s_page, (int)rc);
+    }
+    const int per_tile = R_ROWS / A.per;
+    const cuuint64_t q_size[3] = {(cuuint64_t)head_dim, (cuuint64_t)A.nq, (cuuint64_t)A.T}, q_stride[2] = {(cuuint64_t)(A.nq > 1 ? A.q_head * 2 : head_dim * 2), (cuuint64_t)(A.T > 1 ? A.q_tok * 2 : A.nq * head_dim * 2)};
+    const cuuint32_t q_box[3] = {64, (cuuint32_t)A.per, (cuuint32_t)per_tile};
+    const CUresult rc = encode(&M->q, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(A.q), q_size, q_stride, q_box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (rc != CUDA_SUCCESS) return vfail(MK_ERR_CUDA, "mk_attend: no tensor map for query strides %lld, %lld elements (error %d)", A.q_tok, A.q_head, (int)rc);
+    return MK_OK;
+}
+
 template <int HD, int KIND>
 static int launch_one(const AttendArgs& A, cudaStream_t st) {
     using L = RowsLayout<HD, KIND>;
@@ -612,8 +679,14 @@ static int launch_one(const AttendArgs& A, cudaStream_t st) {
     const int per_tile = R_ROWS / A.per;
     // every request rounds up once
     const long long blocks = (long long)A.T / per_tile + (A.T < A.R ? A.T : A.R);
+    Maps M;
+    if (KIND == K_INT4) memset(&M, 0, sizeof M);
+    else {
+        const int rc = make_maps(A, HD, KIND == K_F16, &M);
+        if (rc != MK_OK) return rc;
+    }
     MKV_CUDA(cudaFuncSetAttribute(attend_rows<HD, KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    MKV_CUDA(launch(attend_rows<HD, KIND>, dim3((unsigned)blocks, A.nkv), L::THREADS, smem, 1, false, st, A));
+    MKV_CUDA(launch(attend_rows<HD, KIND>, dim3((unsigned)blocks, A.nkv), L::THREADS, smem, 1, false, st, A, M));
     return MK_OK;
 }
 template <int HD>

@@ -82,6 +82,7 @@ inline const char* bad_cache(const mk_cache& c) {
     if (!c.k || !c.v || !aligned(c.k, 16) || !aligned(c.v, 16)) return "cache address (16-byte aligned)";
     if (c.type == MKV_INT4) return !c.k_scales || !c.v_scales || !aligned(c.k_scales, 16) || !aligned(c.v_scales, 16) ? "scales (16-byte aligned)" : nullptr;
     if (c.s_page < 0 || c.s_head < 0 || c.s_pos < 0 || c.s_page % 8 || c.s_head % 8 || c.s_pos % 8) return "cache strides (multiples of 8 elements)";
+    if ((c.pages > 1 && !c.s_page) || (c.kv_heads > 1 && !c.s_head) || !c.s_pos) return "cache strides (rows on top of one another)";
     return nullptr;
 }
 
