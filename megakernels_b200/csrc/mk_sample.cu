@@ -4,12 +4,13 @@
 // are read from memory once; everything after that is passes over shared memory with one exchange between the CTAs each.
 //
 //   keep = a prefix of the candidates in the order (key falling, index rising).  A prefix is a key and, among the equals of that
-//   key, how many of them (`need`), the lowest indexes first.  top-k wants the prefix of k candidates, top-p the shortest prefix whose weight reaches
-//   p times that of the first prefix: both are one search for the place where a running sum (of ones, or of weights) over falling keys
-//   reaches a target.  `search` narrows an interval of keys: 256 bins over it, counts and weights per bin summed over the cluster,
-//   the bin that holds the place becomes the interval.  The first level's bins are equal steps of the value (logits crowd into few octaves, so
-//   bins by leading bits would make all lanes add to the same few), later ones equal steps of the key (at most four of those).
-//   A bin whose members all belong to the prefix ends the search.
+// key, how many of them (`need`), the lowest indexes first.  top-k wants the prefix of k candidates, top-p the shortest prefix whose weight reaches
+// p times that of the first prefix: both are one search for the place where a running sum (of ones, or of weights) over falling keys
+// reaches a target.  `search` narrows an interval of keys.  First by a handful of cuts of the value, whose sums stay in registers: they leave a few hundred
+// candidates of most rows, where adding all of them to bins in shared memory would cost more than the rest of the call.  Then by 256 bins over what is left, counts
+// and weights summed over the cluster, the bin that holds the place becoming the interval: equal steps of the value first (by leading bits
+// all lanes would add to the same few), then of the key.
+// An interval whose members all belong to the prefix ends the search.
 //
 // Weights are exp in 64 bits, counted in steps of 2^-44: integer sums, the same in any order, so a border falls the same way whatever the
 // split.  (32-bit weights would move a border of a flat row of 250000 candidates once in some hundred rows.)
@@ -36,15 +37,20 @@ struct SampleArgs {
 struct Bins {
     uint32_t count[S_BINS], lo[S_BINS], hi[S_BINS];        // weights as two words
 };
-struct Shared {
+constexpr int S_CUTS = 5;                // intervals of one round of cuts
+struct alignas(16) Shared {              // (the keys behind it are written sixteen bytes at a time)
+    double powers[32];                   // 2^(i / 32)
     Bins bins[2];
     u64 merged_w[S_BINS];
     uint32_t merged_n[S_BINS];
     u64 warp_w[S_WARPS];
     uint32_t warp_n[S_WARPS];
+    u64 cut_w[S_WARPS][S_CUTS];
+    uint32_t cut_n[S_WARPS][S_CUTS];
     // what every CTA of the cluster writes into every other one
     uint32_t key_of[S_RANKS], live_of[S_RANKS], ties_of[S_RANKS], kept_of[S_RANKS];
-    u64 weight_of[S_RANKS];
+    u64 weight_of[S_RANKS], cut_w_of[2][S_CUTS][S_RANKS];
+    uint32_t cut_n_of[2][S_CUTS][S_RANKS];
     u64 above;
     uint32_t bin, bin_n, border[2];
 };
@@ -79,6 +85,8 @@ __device__ __forceinline__ void remote_store(u64* p, int rank, u64 v) {
     asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(remote(p, rank)), "l"(v) : "memory");
 }
 
+__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
 constexpr uint32_t LOWEST = 0x00800000u;                   // the key of the lowest finite value
 // Keys order as the values do; 0 is kept for what is masked (-inf, NaN).  -0 counts as 0.
 __device__ __forceinline__ uint32_t key_of(float x) {
@@ -88,64 +96,154 @@ __device__ __forceinline__ uint32_t key_of(float x) {
 }
 __device__ __forceinline__ float value_of(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7FFFFFFFu : ~key); }
 
-// The weight of a key in steps of 2^-44.
-__device__ __forceinline__ u64 weight(uint32_t key, uint32_t top, double inv_t) {
+// The weight of a key in steps of 2^-44: exp by a table of 2^(i / 32) and a polynomial of degree 5 on |r| <= ln 2 / 64 (the table-driven method of Tang, 1989; the
+// terms left out are below 2^-48), rounded to a whole number by an addition of 2^52.
+__device__ __forceinline__ u64 weight(uint32_t key, uint32_t top, double inv_t, const double* powers) {
     if (key == top) return 1ull << 44;                      // also where the largest is infinite
     const double y = ((double)value_of(key) - (double)value_of(top)) * inv_t;
-    return y < -31.5 ? 0ull : (u64)__double2ll_rn(exp(y) * 17592186044416.0);
+    if (!(y >= -31.5)) return 0ull;
+    const double magic = 6755399441055744.0, t = fma(y, 46.16624130844683, magic);     // 32 / ln 2; 1.5 * 2^52
+    const int n = __double2loint(t);
+    const double k = t - magic;
+    double r = fma(k, -0.021660849392446835, y);            // ln 2 / 32 to 38 bits (k has 11: exact), and the rest of it
+    r = fma(k, -5.1456092446553379e-14, r);
+    double e = fma(r, 1.0 / 120, 1.0 / 24);
+    e = fma(e, r, 1.0 / 6);
+    e = fma(e, r, 0.5);
+    e = fma(e, r, 1.0);
+    e = fma(e, r, 1.0) * powers[n & 31];
+    e = __hiloint2double(__double2hiint(e) + (((n >> 5) + 44) << 20), __double2loint(e));
+    return (u64)(__double_as_longlong(e + 4503599627370496.0) & 0xFFFFFFFFFFFFFll);
 }
+
+static_assert(sizeof(Shared) % 16 == 0, "keys behind it");
 
 struct Place {
     uint32_t key, need;                  // the prefix's last key, and how many of its equals belong to the prefix
+    uint32_t equals;                     // how many there are, where `need` is not all of them
 };
+constexpr uint32_t ALL = 0xFFFFFFFFu;
 
 struct Row {
     Shared* S;
     const uint32_t* keys;
-    int n, rank, ranks, level;           // level: how many exchanges of bins so far (they alternate between two buffers)
+    int n, rank, ranks, level, cuts;     // level, cuts: how many exchanges of bins and of cuts so far (they alternate between two buffers)
     uint32_t top;
     double inv_t;
 };
 
-// One level: bins over keys in [lo, hi], summed over the cluster.  `by_value`: bins are equal steps of the value.
+__device__ __forceinline__ u64 warp_add(u64 v) {
+    // (pieces of 24 bits, so that 32 of them fit a word)
+    const uint32_t a = __reduce_add_sync(~0u, (uint32_t)v & 0xFFFFFFu), b = __reduce_add_sync(~0u, (uint32_t)(v >> 24) & 0xFFFFFFu), c = __reduce_add_sync(~0u, (uint32_t)(v >> 48));
+    return (u64)a + ((u64)b << 24) + ((u64)c << 48);
+}
+
+// The bin of a key of the interval that ends with `hi`: equal steps of the value or of the key.  (The last one of values takes what rounding leaves over.)
 __device__ __forceinline__ int bin_of(uint32_t key, uint32_t hi, float hi_value, float per_value, uint32_t step, bool by_value) {
     if (by_value) return min(S_BINS - 1, (int)((hi_value - value_of(key)) * per_value));
     return (int)((hi - key) / step);
 }
 
-// The prefix at which the running sum of ones (weights == false) or weights reaches `target` > 0, over candidates with keys in [lo, hi] (and of
-// `lo` only `lo_need`, if weighted); the sum over all of them is at least the target.
+// The prefix at which the running sum of ones (weights == false) reaches `share` > 0, or the running sum of weights `share` times that of
+// the candidates down to `within` (of its equals only `within.need`).  The sum over all candidates is at least the target.
 template <bool WEIGHTS>
-__device__ Place search(Row& R, uint32_t lo, uint32_t hi, double target, uint32_t lo_need) {
+__device__ Place search(Row& R, Place within, double share) {
     Shared& S = *R.S;
-    const int tid = threadIdx.x;
-    const uint32_t floor_key = lo;
-    double left = target;                                    // what the candidates above the interval leave of it
-    u64 above = 0;
-    bool by_value = value_of(hi) < INFINITY;                 // the first level
-    for (;;) {
-        if (lo == hi) break;
+    const int tid = threadIdx.x, lane = tid & 31;
+    uint32_t lo = within.key, hi = R.top;
+    double target = share;                                   // in ones, or in steps of 2^-44
+    u64 above = 0;                                           // the sum above the interval
+    const u64 floor_w = WEIGHTS ? weight(within.key, R.top, R.inv_t, S.powers) : 0ull, excess = within.need == ALL ? 0ull : (u64)(within.equals - within.need);
+    uint32_t members = 0;
+    {
+        // ---- the cuts: 1, 3, 6 and 12 temperatures below the largest
+        const double t = 1.0 / R.inv_t, top = (double)value_of(hi);
+        uint32_t cut[S_CUTS];
+#pragma unroll
+        for (int j = 0; j < S_CUTS - 1; j++) {
+            const double below[S_CUTS - 1] = {1, 3, 6, 12};
+            cut[j] = min(max(lo, key_of((float)(top - t * below[j]))), hi);              // (an infinite largest: its own key)
+        }
+        cut[S_CUTS - 1] = lo;
+        u64 w[S_CUTS] = {};
+        uint32_t n[S_CUTS] = {};
+        for (int e = tid; e < R.n; e += S_THREADS) {
+            const uint32_t key = R.keys[e];
+            if (key < lo) continue;
+            const u64 x = WEIGHTS ? weight(key, R.top, R.inv_t, S.powers) : 0ull;
+#pragma unroll
+            for (int j = 0; j < S_CUTS; j++)                 // running: down to every cut
+                if (key >= cut[j]) n[j]++, w[j] += x;
+        }
+#pragma unroll
+        for (int j = 0; j < S_CUTS; j++) {
+            const uint32_t a = __reduce_add_sync(~0u, n[j]);
+            const u64 b = WEIGHTS ? warp_add(w[j]) : 0ull;
+            if (lane == 0) S.cut_n[tid >> 5][j] = a, S.cut_w[tid >> 5][j] = b;
+        }
+        __syncthreads();
+        const int buffer = R.cuts++ & 1;
+        if (tid < S_CUTS * R.ranks) {
+            const int j = tid / R.ranks, to = tid - j * R.ranks;
+            uint32_t a = 0;
+            u64 b = 0;
+            for (int x = 0; x < S_WARPS; x++) a += S.cut_n[x][j], b += S.cut_w[x][j];
+            remote_store(&S.cut_n_of[buffer][j][R.rank], to, a);
+            if (WEIGHTS) remote_store(&S.cut_w_of[buffer][j][R.rank], to, b);
+        }
+        cluster_barrier();
+        u64 sum_w[S_CUTS];
+        uint32_t sum_n[S_CUTS];
+#pragma unroll
+        for (int j = 0; j < S_CUTS; j++) {
+            sum_w[j] = 0, sum_n[j] = 0;
+            for (int r = 0; r < R.ranks; r++) {
+                sum_n[j] += S.cut_n_of[buffer][j][r];
+                if (WEIGHTS) sum_w[j] += S.cut_w_of[buffer][j][r];
+            }
+        }
+        if (WEIGHTS) {
+            target = share * (double)(sum_w[S_CUTS - 1] - excess * floor_w);
+            if (!(target > 0)) return {R.top, 1u, 0u};       // the first candidate always stays
+        }
+        bool found = false;
+#pragma unroll
+        for (int j = 0; j < S_CUTS; j++) {
+            if (found || cut[j] > hi) continue;
+            const u64 upto = WEIGHTS ? sum_w[j] : (u64)sum_n[j];
+            if ((double)upto >= target || cut[j] == lo) {
+                members = sum_n[j] - (j ? sum_n[j - 1] : 0u);
+                if (!WEIGHTS && (double)upto == target) return {cut[j], ALL, 0u};
+                lo = cut[j], found = true;
+            } else {
+                above = upto;
+                hi = cut[j] - 1;                             // (above lo, which the last cut is)
+            }
+        }
+        if (members == 1) return {lo, ALL, 0u};
+    }
+    while (lo < hi) {
         Bins& B = S.bins[R.level & 1];
         R.level++;
-        // equal steps of the value reach down to a weight of exp(-32), the last bin holds the rest
-        const float hi_value = value_of(hi), per_value = (float)(S_BINS / 32 * R.inv_t);
+        // equal steps of the value where the interval is one of ordinary values and many keys, else of the key
+        const float hi_value = value_of(hi), width = hi_value - value_of(lo), per_value = (float)S_BINS / width;
+        const bool by_value = (double)width * R.inv_t < 64 && hi - lo > 1u << 16 && per_value < 1e30f;
         const uint32_t step = (hi - lo) / S_BINS + 1;
-        const bool value_bins = by_value && per_value < 1e30f;
         for (int i = tid; i < S_BINS; i += S_THREADS) B.count[i] = B.lo[i] = B.hi[i] = 0;
         __syncthreads();
         for (int e = tid; e < R.n; e += S_THREADS) {
             const uint32_t key = R.keys[e];
             if (key < lo || key > hi) continue;
-            const int b = bin_of(key, hi, hi_value, per_value, step, value_bins);
+            const int b = bin_of(key, hi, hi_value, per_value, step, by_value);
             atomicAdd(&B.count[b], 1u);
             if (WEIGHTS) {
-                const u64 w = weight(key, R.top, R.inv_t);
+                const u64 w = weight(key, R.top, R.inv_t, S.powers);
                 const uint32_t w_lo = (uint32_t)w, old = atomicAdd(&B.lo[b], w_lo), w_hi = (uint32_t)(w >> 32) + (old + w_lo < old);
                 if (w_hi) atomicAdd(&B.hi[b], w_hi);
             }
         }
         cluster_barrier();
-        // every CTA adds up all of them (8 to 12 KB); the buffer is written again two levels on, behind the next barrier
+        // every CTA adds up all of them (1 to 3 KB each); the buffer is written again two levels on, behind the next barrier
         for (int b = tid; b < S_BINS; b += S_THREADS) {
             uint32_t n = 0;
             u64 w = 0;
@@ -168,14 +266,14 @@ __device__ Place search(Row& R, uint32_t lo, uint32_t hi, double target, uint32_
                 const u64 v = __shfl_up_sync(~0u, upto, d);
                 if (tid >= d) upto += v;
             }
-            const uint32_t reached = __ballot_sync(~0u, (double)(above + upto) >= left);
+            const uint32_t reached = __ballot_sync(~0u, (double)(above + upto) >= target);
             const int who = reached ? __ffs(reached) - 1 : 31;
             if (tid == who) {
                 u64 run = above + upto - mine;
                 int b = tid * 8;
                 for (; b < tid * 8 + 7; b++) {
                     const u64 next = run + (WEIGHTS ? S.merged_w[b] : (u64)S.merged_n[b]);
-                    if ((double)next >= left) break;
+                    if ((double)next >= target) break;
                     run = next;
                 }
                 S.bin = b;
@@ -184,76 +282,93 @@ __device__ Place search(Row& R, uint32_t lo, uint32_t hi, double target, uint32_
             }
         }
         __syncthreads();
-        const int b = (int)S.bin;
+        const uint32_t b = S.bin;
         above = S.above;
-        const uint32_t members = S.bin_n;
+        members = S.bin_n;
         __syncthreads();
-        // the bin's interval of keys
-        if (value_bins) {
-            // bin_of falls as the key rises: the smallest keys with a bin of b or less, and of b - 1 or less
+        if (by_value) {
+            // bin_of falls as the key rises: the smallest keys with a bin of b or less, and of b - 1 or less, by 32-fold division
             if (tid < 64) {
-                const int want = tid < 32 ? b : b - 1, at = tid & 31;
+                const int want = (int)b - (tid >> 5);
                 uint32_t l = lo, h = hi;                      // (hi itself is in bin 0; for b = 0 the second border is not used)
                 while (l < h) {
-                    const uint32_t part = (h - l) / 32 + 1, m = l + part * at;
-                    const bool beyond = m >= h || m < l;
-                    const uint32_t yes = __ballot_sync(~0u, beyond || bin_of(m, hi, hi_value, per_value, step, true) <= want);
+                    const uint32_t part = (h - l) / 32 + 1, m = l + part * lane;
+                    const uint32_t yes = __ballot_sync(~0u, m >= h || m < l || bin_of(m, hi, hi_value, per_value, step, true) <= want);
                     const int j = yes ? __ffs(yes) - 1 : 32;
-                    const uint32_t new_h = j < 32 && l + part * j < h && l + part * j >= l ? l + part * j : h;
-                    l = j > 0 ? l + part * (j - 1) + 1 : l;
-                    h = new_h;
-                    if (l > h) l = h;
+                    const uint32_t at = l + part * j;
+                    if (j < 32 && at < h && at >= l) h = at;
+                    if (j > 0) l = min(h, l + part * (j - 1) + 1);
                 }
-                if (at == 0) S.border[tid >> 5] = l;
+                if (lane == 0) S.border[tid >> 5] = l;
             }
             __syncthreads();
             lo = S.border[0];
             if (b > 0) hi = max(lo, S.border[1] - 1);
         } else {
-            const uint32_t top = hi - (uint32_t)b * step, width = step - 1;
-            lo = top - lo > width ? top - width : lo;
+            const uint32_t top = hi - b * step;
+            lo = top - lo >= step ? top - step + 1 : lo;
             hi = top;
         }
-        by_value = false;
-        if (members == 1 || (!WEIGHTS && (double)(above + members) == left)) return {lo, 0xFFFFFFFFu};   // all of them: no key is cut
+        if (members == 1 || (!WEIGHTS && (double)(above + members) == target)) return {lo, ALL, 0u};     // all of them: no key is cut
     }
     // one key: how many of its equals
-    if (!WEIGHTS) return {lo, (uint32_t)(left - (double)above)};
-    const u64 w = weight(lo, R.top, R.inv_t);
     uint32_t n = 1;
-    if (w) {
-        n = (uint32_t)fmin(fmax(ceil((left - (double)above) / (double)w), 1.0), 4294967040.0);
-        if (n > 1 && (double)(above + (u64)(n - 1) * w) >= left) n--;              // the division's rounding
-        else if ((double)(above + (u64)n * w) < left) n++;
+    if (!WEIGHTS) n = (uint32_t)(target - (double)above);
+    else {
+        const u64 w = weight(lo, R.top, R.inv_t, S.powers);
+        if (w) {
+            n = (uint32_t)fmin(fmax(ceil((target - (double)above) / (double)w), 1.0), 4294967040.0);
+            if (n > 1 && (double)(above + (u64)(n - 1) * w) >= target) n--;                // the division's rounding
+            else if ((double)(above + (u64)n * w) < target) n++;
+        }
+        if (lo == within.key && within.need != ALL) n = min(n, within.need);
     }
-    return {lo, lo == floor_key && n > lo_need ? lo_need : n};
+    return {lo, n >= members ? ALL : n, members};
 }
 
-__device__ __forceinline__ u64 warp_add(u64 v) {
-#pragma unroll
-    for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(~0u, v, d);
-    return v;
-}
-
-static __global__ void __launch_bounds__(S_THREADS) sample_rows(const __grid_constant__ SampleArgs A) {
+static __global__ void __launch_bounds__(S_THREADS, 2) sample_rows(const __grid_constant__ SampleArgs A) {
     extern __shared__ __align__(16) uint8_t smem[];
     Shared& S = *reinterpret_cast<Shared*>(smem);
     uint32_t* keys = reinterpret_cast<uint32_t*>(smem + sizeof(Shared));
     const int ranks = nctarank(), rank = ctarank(), row = blockIdx.x / ranks, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int first = rank * A.piece, n = max(0, min(A.vocab - first, A.piece));
+    if (tid < 32) S.powers[tid] = exp2((double)tid * (1.0 / 32));
     // ---- the piece as keys, its largest and how many are not masked
     uint32_t best = 0, live = 0;
     {
         const long long base = (long long)row * A.stride + first;
-        for (int e = tid; e < n; e += S_THREADS) {
-            const float x = A.type == MKV_F32 ? __ldg(reinterpret_cast<const float*>(A.logits) + base + e)
-                                              : (A.type == MKV_BF16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(A.logits)[base + e])
-                                                                    : __half2float(reinterpret_cast<const __half*>(A.logits)[base + e]));
+        auto take = [&](float x) {
             const uint32_t key = key_of(x);
-            keys[e] = key;
             best = max(best, key);
             live += key != 0;
-        }
+            return key;
+        };
+        auto read = [&](auto zero) {
+            typedef decltype(zero) T;
+            constexpr int V = 16 / sizeof(T);
+            const T* src = reinterpret_cast<const T*>(A.logits) + base;
+            auto value = [](T x) {
+                if constexpr (sizeof(T) == 4) return (float)x;
+                else return to_float(x);
+            };
+            const int wide = ((uintptr_t)src & 15) == 0 ? n / V : 0;      // rows that do not start on a 16-byte boundary are read one by one
+#pragma unroll 4
+            for (int e = tid; e < wide; e += S_THREADS) {
+                const uint4 raw = __ldg(reinterpret_cast<const uint4*>(src) + e);
+                alignas(16) T x[V];
+                *reinterpret_cast<uint4*>(x) = raw;
+                uint32_t k[V];
+#pragma unroll
+                for (int i = 0; i < V; i++) k[i] = take(value(x[i]));
+#pragma unroll
+                for (int i = 0; i < V; i += 4) *reinterpret_cast<uint4*>(keys + e * V + i) = make_uint4(k[i], k[i + 1], k[i + 2], k[i + 3]);
+            }
+#pragma unroll 4
+            for (int e = wide * V + tid; e < n; e += S_THREADS) keys[e] = take(value(src[e]));
+        };
+        if (A.type == MKV_F32) read(0.f);
+        else if (A.type == MKV_BF16) read(__nv_bfloat16());
+        else read(__half());
     }
     best = __reduce_max_sync(~0u, best);
     live = __reduce_add_sync(~0u, live);
@@ -276,15 +391,18 @@ static __global__ void __launch_bounds__(S_THREADS) sample_rows(const __grid_con
     int k = A.top_k[row];
     const bool greedy = !(t > 0.f);
     if (greedy) k = 1;
-    Row R = {&S, keys, n, rank, ranks, 0, top, greedy ? 1.0 : 1.0 / (double)t};
+    Row R = {&S, keys, n, rank, ranks, 0, 0, top, greedy ? 1.0 : 1.0 / (double)t};
     // ---- the prefix
-    Place at = {LOWEST, 0xFFFFFFFFu};                         // all that is not masked
-    if (k == 1) at = {top, 1u};
-    else if (k > 1 && (uint32_t)k < total) at = search<false>(R, LOWEST, top, (double)k, 0u);
-    // how many equals of the cut key every CTA holds, and the weight of the prefix
-    auto ties = [&](uint32_t key, uint32_t* before) {
+    Place at = {LOWEST, ALL, 0u};                             // all that is not masked
+    const bool one = k == 1;
+    if (one) at = {top, 1u, 0u};
+    else if (k > 1 && (uint32_t)k < total) at = search<false>(R, at, (double)k);
+    if (p < 1.f && !one) at = search<true>(R, at, (double)p);
+    // of the equals of the cut key, the lowest indexes: how many lie in the CTAs in front
+    uint32_t before = 0;
+    if (at.need != ALL) {
         uint32_t mine = 0;
-        for (int e = tid; e < n; e += S_THREADS) mine += keys[e] == key;
+        for (int e = tid; e < n; e += S_THREADS) mine += keys[e] == at.key;
         mine = __reduce_add_sync(~0u, mine);
         __syncthreads();
         if (lane == 0) S.warp_n[warp] = mine;
@@ -295,40 +413,11 @@ static __global__ void __launch_bounds__(S_THREADS) sample_rows(const __grid_con
             remote_store(&S.ties_of[rank], tid, l);
         }
         cluster_barrier();
-        uint32_t all = 0;
-        *before = 0;
-        for (int r = 0; r < ranks; r++) {
-            if (r < rank) *before += S.ties_of[r];
-            all += S.ties_of[r];
-        }
-        return all;
-    };
-    if (p < 1.f && !(at.key == top && at.need == 1u)) {
-        u64 mine = 0;
-        for (int e = tid; e < n; e += S_THREADS)
-            if (keys[e] > at.key || (keys[e] == at.key && at.need == 0xFFFFFFFFu)) mine += weight(keys[e], top, R.inv_t);
-        mine = warp_add(mine);
-        __syncthreads();
-        if (lane == 0) S.warp_w[warp] = mine;
-        __syncthreads();
-        if (tid < ranks) {
-            u64 l = 0;
-            for (int w = 0; w < S_WARPS; w++) l += S.warp_w[w];
-            remote_store(&S.weight_of[rank], tid, l);
-        }
-        cluster_barrier();
-        u64 all = 0;
-        for (int r = 0; r < ranks; r++) all += S.weight_of[r];
-        if (at.need != 0xFFFFFFFFu) all += (u64)at.need * weight(at.key, top, R.inv_t);
-        const double target = (double)p * (double)all;
-        // the first candidate always stays
-        at = target > 0 ? search<true>(R, at.key, top, target, at.need) : Place{top, 1u};
+        for (int r = 0; r < rank; r++) before += S.ties_of[r];
     }
-    uint32_t before = 0;
-    if (at.need != 0xFFFFFFFFu && ties(at.key, &before) <= at.need) at.need = 0xFFFFFFFFu;
     // ---- weights of the kept ones, in index order: a run of the piece per warp
     const int per_warp = ((n + S_WARPS - 1) / S_WARPS + 31) & ~31, w0 = min(n, warp * per_warp), w1 = min(n, w0 + per_warp);
-    if (at.need != 0xFFFFFFFFu) {
+    if (at.need != ALL) {
         uint32_t mine = 0;
         for (int e = w0 + lane; e < w1; e += 32) mine += keys[e] == at.key;
         mine = __reduce_add_sync(~0u, mine);
@@ -343,11 +432,11 @@ static __global__ void __launch_bounds__(S_THREADS) sample_rows(const __grid_con
         const uint32_t key = e < w1 ? keys[e] : 0u;
         stays = key > at.key;
         const uint32_t equal = __ballot_sync(~0u, key == at.key && key != 0);
-        if (key == at.key && key != 0) stays = at.need == 0xFFFFFFFFu || seen + __popc(equal & ((1u << lane) - 1)) < at.need;
+        if (key == at.key && key != 0) stays = at.need == ALL || seen + __popc(equal & ((1u << lane) - 1)) < at.need;
         seen += __popc(equal);
         u64 w = 0;
         if (stays) {
-            w = weight(key, top, R.inv_t);
+            w = weight(key, top, R.inv_t, S.powers);
             stays = (double)w >= floor_w;
         }
         return stays ? w : 0ull;
@@ -432,9 +521,11 @@ extern "C" int mk_sample(const mk_sample_args* a, void* stream) {
     A.top_k = reinterpret_cast<const int*>(a->top_k);
     A.ids = reinterpret_cast<int*>(a->ids), A.kept = reinterpret_cast<int*>(a->kept), A.logprobs = reinterpret_cast<float*>(a->logprobs);
     A.stride = a->stride, A.rows = a->rows, A.vocab = a->vocab, A.type = a->type;
-    // CTAs of a row: as many as keep a piece at 2048 logits or more
+    // CTAs of a row: more of them shorten its passes, but clusters wait for room (one of 16 takes a whole GPC's SMs), so all rows together take about
+    // 256 CTAs, and more only where a piece would be longer than 20000 logits.  Greedy, us: 64 rows of 30000 with 2, 4, 8, 16 CTAs each 18, 15, 20, 39;
+    // of 151936 with 4, 8, 16 64, 41, 55; of 248320 with 8, 16 87, 73; one row of 151936 with 4, 8, 16 24, 17, 12.
     int ranks = 1;
-    while (ranks < S_RANKS && a->vocab > ranks * 2048) ranks *= 2;
+    while (ranks < S_RANKS && a->vocab > ranks * 2048 && ((int64_t)a->rows * ranks * 2 <= 256 || a->vocab > ranks * 20000)) ranks *= 2;
     A.piece = ((a->vocab + ranks - 1) / ranks + 31) & ~31;
     const size_t smem = sizeof(Shared) + (size_t)A.piece * 4;
     MKV_CUDA(cudaFuncSetAttribute(sample_rows, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
