@@ -63,6 +63,12 @@ __device__ __forceinline__ long long build_line(const AttendArgs& A, long long* 
     return all;
 }
 
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 template <int HD, int KIND> struct Layout {
     static constexpr int ROW = KIND == K_INT4 ? HD / 2 : HD * 2;                   // bytes of a cache row
     static constexpr int META = KIND == K_INT4 ? HD / 64 * 4 : 0;
@@ -82,6 +88,13 @@ template <int ROW> __device__ __forceinline__ int staged(int row, int byte) {
         return row * ROW + (byte ^ (f << 4));
     } else if constexpr (ROW == 64) return row * ROW + (byte ^ ((row >> 2 & 3) << 4));
     else return row * ROW + (byte ^ ((row >> 2 & 1) << 4));
+}
+
+// A row's (scale, low) pairs.
+template <int G> __device__ __forceinline__ void load_scales(uint32_t (&m)[G], const uint8_t* p) {
+    if constexpr (G == 4) *reinterpret_cast<uint4*>(m) = *reinterpret_cast<const uint4*>(p);
+    else if constexpr (G == 2) *reinterpret_cast<uint2*>(m) = *reinterpret_cast<const uint2*>(p);
+    else m[0] = *reinterpret_cast<const uint32_t*>(p);
 }
 
 template <int HD, int KIND>
@@ -195,29 +208,50 @@ static __global__ void __launch_bounds__(Layout<HD, KIND>::WARPS * 32, 1) attend
             const int page = n < A.max_pages ? __ldg(A.table + r * A.table_stride + n) : -1;
             return page >= 0 && page < A.pages ? page : -1;
         };
+        // this lane's pieces of a tile: row0, row0 + AT_ONCE, ... (a 4-bit row's address is a compile-time distance from the one before)
+        constexpr int P = L::ROW / 16, AT_ONCE = 32 / P > 0 ? 32 / P : 1, STEPS = A_KEYS * P / 32;
+        const int row_l = P <= 32 ? lane / P : 0, byte_l = P <= 32 ? (lane % P) * 16 : lane * 16;
+        auto place = [&](int j) { return P <= 32 ? staged<L::ROW>(row_l + j * AT_ONCE, byte_l) : staged<L::ROW>(j * 32 / P, byte_l + j * 32 % P * 16); };
         auto fetch = [&](int tile, int slot) {
             if (tile < t1) {
                 const int key0 = key0_of(tile), page = page_of(key0), off = key0 & ((1 << A.page_shift) - 1);
                 if (page >= 0) {
                     const uint32_t dst = ring_u + slot * L::SLOT;
-                    const long long base = page * A.s_page + head * A.s_head + off * A.s_pos;
-                    constexpr int P = L::ROW / 16;                                 // pieces of a row
-#pragma unroll
-                    for (int j = 0; j < A_KEYS * P / 32; j++) {
-                        const int i = j * 32 + lane, row = i / P, byte = (i % P) * 16, key = key0 + row;
-                        const bool live = key <= pos_hi && (key >= win_lo || key < A.sinks);
-                        const long long o2 = base + row * A.s_pos + byte;
-                        cp16(dst + staged<L::ROW>(row, byte), A.k + o2, live);
-                        cp16(dst + A_KEYS * L::ROW + staged<L::ROW>(row, byte), A.v + o2, live);
-                    }
+                    const long long s_pos = I4 ? (long long)L::ROW : A.s_pos, at = page * A.s_page + head * A.s_head + off * s_pos + row_l * s_pos + byte_l;
+                    const uint8_t *k = A.k + at, *v = A.v + at;
+                    auto seen = [&](int row) { return key0 + row <= pos_hi && (key0 + row >= win_lo || key0 + row < A.sinks); };
+                    const bool all = key0 + A_KEYS - 1 <= pos_hi && (key0 >= win_lo || key0 + A_KEYS <= A.sinks);
+                    const uint8_t* meta = nullptr;
+                    uint32_t meta_to = 0;
                     if constexpr (I4) {
-                        const long long row0_ = (((long long)page * A.nkv + head) << A.page_shift) + off;
-                        const int row = lane & 15, key = key0 + row;
-                        const bool live = key <= pos_hi && (key >= win_lo || key < A.sinks);
-                        const uint8_t* src = (lane < 16 ? A.ks : A.vs) + (row0_ + row) * L::META;
-                        const uint32_t to = dst + A_KEYS * 2 * L::ROW + (lane < 16 ? 0 : A_KEYS * L::META) + row * L::META;
-                        if constexpr (L::META == 16) cp16(to, src, live);
-                        else cp_small<L::META>(to, src, live);
+                        const long long row = (((long long)page * A.nkv + head) << A.page_shift) + off + (lane & 15);
+                        meta = (lane < 16 ? A.ks : A.vs) + row * L::META;
+                        meta_to = dst + A_KEYS * 2 * L::ROW + lane * L::META;
+                    }
+                    if (all) {
+#pragma unroll
+                        for (int j = 0; j < STEPS; j++) {
+                            const long long o2 = P <= 32 ? j * AT_ONCE * s_pos : (j * 32 / P) * s_pos + j * 32 % P * 16;
+                            cp16(dst + place(j), k + o2);
+                            cp16(dst + A_KEYS * L::ROW + place(j), v + o2);
+                        }
+                        if constexpr (I4) {
+                            if constexpr (L::META == 16) cp16(meta_to, meta);
+                            else cp_small<L::META>(meta_to, meta, true);
+                        }
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < STEPS; j++) {
+                            const long long o2 = P <= 32 ? j * AT_ONCE * s_pos : (j * 32 / P) * s_pos + j * 32 % P * 16;
+                            const bool live = seen(P <= 32 ? row_l + j * AT_ONCE : j * 32 / P);
+                            cp16(dst + place(j), k + o2, live);
+                            cp16(dst + A_KEYS * L::ROW + place(j), v + o2, live);
+                        }
+                        if constexpr (I4) {
+                            const bool live = seen(lane & 15);
+                            if constexpr (L::META == 16) cp16(meta_to, meta, live);
+                            else cp_small<L::META>(meta_to, meta, live);
+                        }
                     }
                 }
             }
@@ -243,6 +277,9 @@ static __global__ void __launch_bounds__(Layout<HD, KIND>::WARPS * 32, 1) attend
             float sc[4] = {0.f, 0.f, 0.f, 0.f};
             if constexpr (I4) {
                 const uint8_t* ms = ks + A_KEYS * 2 * L::ROW;
+                uint32_t ma[G], mb[G];
+                load_scales<G>(ma, ms + ka * L::META);
+                load_scales<G>(mb, ms + (ka + 2) * L::META);
                 // a row's words are [8][G]: lane t multiplies words (2 t, .) and (2 t + 1, .)
                 uint32_t wa[2 * G], wb[2 * G];
 #pragma unroll
@@ -268,8 +305,7 @@ static __global__ void __launch_bounds__(Layout<HD, KIND>::WARPS * 32, 1) attend
                         mma<false>(x, codes<0>(a), codes<0>(b), codes<1>(a), codes<1>(b), qf[c2 * 4 + w * 2][0], qf[c2 * 4 + w * 2][1]);
                         mma<false>(x, codes<2>(a), codes<2>(b), codes<3>(a), codes<3>(b), qf[c2 * 4 + w * 2 + 1][0], qf[c2 * 4 + w * 2 + 1][1]);
                     }
-                    const uint32_t ma = *reinterpret_cast<const uint32_t*>(ms + ka * L::META + c2 * 4), mb = *reinterpret_cast<const uint32_t*>(ms + (ka + 2) * L::META + c2 * 4);
-                    const float sa = __uint_as_float(ma << 16), la = __uint_as_float(ma & 0xFFFF0000u), sb = __uint_as_float(mb << 16), lb = __uint_as_float(mb & 0xFFFF0000u);
+                    const float sa = __uint_as_float(ma[c2] << 16), la = __uint_as_float(ma[c2] & 0xFFFF0000u), sb = __uint_as_float(mb[c2] << 16), lb = __uint_as_float(mb[c2] & 0xFFFF0000u);
                     sc[0] = fmaf(sa, x[0], fmaf(la, qsum[c2][0], sc[0]));
                     sc[1] = fmaf(sa, x[1], fmaf(la, qsum[c2][1], sc[1]));
                     sc[2] = fmaf(sb, x[2], fmaf(lb, qsum[c2][0], sc[2]));
@@ -295,21 +331,19 @@ static __global__ void __launch_bounds__(Layout<HD, KIND>::WARPS * 32, 1) attend
                 if (!whole && (key > pos[j] || (A.window && key <= pos[j] - A.window && key >= A.sinks))) sc[i] = -INFINITY;
             }
             float top[2] = {fmaxf(sc[0], sc[2]), fmaxf(sc[1], sc[3])};
-            float vmax = 0.f;
-            uint32_t vm[4][G];
+            // 4 bits: the scales of this lane's four keys (4 t ... 4 t + 3), and the largest of scales and lows as the bits they are (bf16 without a sign orders
+            // as a whole number does)
+            uint32_t vm[4][G], vbits = 0u;
+            const uint8_t* const ms_v = ks + A_KEYS * (2 * L::ROW + L::META);
             if constexpr (I4) {
-                // the scales of this lane's four keys (4 t ... 4 t + 3)
-                const uint8_t* ms = ks + A_KEYS * (2 * L::ROW + L::META);
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const uint32_t* p = reinterpret_cast<const uint32_t*>(ms + (4 * t + j) * L::META);
+                for (int j = 0; j < 4; j++) load_scales<G>(vm[j], ms_v + (4 * t + j) * L::META);
 #pragma unroll
-                    for (int c2 = 0; c2 < G; c2++) {
-                        vm[j][c2] = p[c2];
-                        vmax = fmaxf(vmax, fmaxf(15.f * __uint_as_float(vm[j][c2] << 16), fabsf(__uint_as_float(vm[j][c2] & 0xFFFF0000u))));
-                    }
-                }
+                for (int j = 0; j < 4; j += 2)
+#pragma unroll
+                    for (int c2 = 0; c2 < G; c2++) vbits = __vimax3_u16x2(vbits, vm[j][c2] & 0x7FFF7FFFu, vm[j + 1][c2] & 0x7FFF7FFFu);
             }
+            const float vmax = fmaxf(15.f * __uint_as_float(vbits << 16), __uint_as_float(vbits & 0xFFFF0000u));
             if (__any_sync(~0u, top[0] > ref[0] + 8.f || top[1] > ref[1] + 8.f || (I4 && vmax > 16.f * v_unit))) {
                 float f[2];
 #pragma unroll
@@ -319,7 +353,7 @@ static __global__ void __launch_bounds__(Layout<HD, KIND>::WARPS * 32, 1) attend
                     m = fmaxf(m, __shfl_xor_sync(~0u, m, 8));
                     m = fmaxf(m, __shfl_xor_sync(~0u, m, 16));
                     m = fmaxf(m, ref[j]);
-                    f[j] = m == -INFINITY ? 1.f : exp2f(ref[j] - m);               // (nothing so far: 0)
+                    f[j] = m == -INFINITY ? 1.f : exp2_fast(ref[j] - m);               // (nothing so far: 0)
                     sum[j] *= f[j];
                     ref[j] = m;
                 }
@@ -343,7 +377,7 @@ static __global__ void __launch_bounds__(Layout<HD, KIND>::WARPS * 32, 1) attend
             float p[4];
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                p[i] = sc[i] == -INFINITY ? 0.f : exp2f(sc[i] - ref[i & 1]);
+                p[i] = exp2_fast(sc[i] - (ref[i & 1] == -INFINITY ? 0.f : ref[i & 1]));     // (-inf: 0)
                 sum[i & 1] += p[i];
             }
             // ---- outputs: rows are dims, this lane's keys 4 t ... 4 t + 3
@@ -357,17 +391,20 @@ static __global__ void __launch_bounds__(Layout<HD, KIND>::WARPS * 32, 1) attend
                     else if constexpr (G == 2) *reinterpret_cast<uint2*>(w[j]) = *reinterpret_cast<const uint2*>(src);
                     else w[j][0] = *reinterpret_cast<const uint32_t*>(src);
                 }
-                uint32_t la = 0u, lb = 0u;
+                // row g of the lows: those of group g (rows past the groups repeat them and go nowhere)
+                uint32_t la, lb;
+                {
+                    float low[4];
+#pragma unroll
+                    for (int j = 0; j < 4; j++) low[j] = __uint_as_float(*reinterpret_cast<const uint32_t*>(ms_v + (4 * t + j) * L::META + (g & (G - 1)) * 4) & 0xFFFF0000u) * v_inv;
+                    la = pack_half(low[0], low[1]), lb = pack_half(low[2], low[3]);
+                }
 #pragma unroll
                 for (int c2 = 0; c2 < G; c2++) {
                     float sv[4];
 #pragma unroll
                     for (int j = 0; j < 4; j++) sv[j] = __uint_as_float(vm[j][c2] << 16) * v_inv;
                     const uint32_t b0 = mul_half2(p0, pack_half(sv[0], sv[1])), b1 = mul_half2(p1, pack_half(sv[2], sv[3]));
-                    if (g == c2) {
-                        la = pack_half(__uint_as_float(vm[0][c2] & 0xFFFF0000u) * v_inv, __uint_as_float(vm[1][c2] & 0xFFFF0000u) * v_inv);
-                        lb = pack_half(__uint_as_float(vm[2][c2] & 0xFFFF0000u) * v_inv, __uint_as_float(vm[3][c2] & 0xFFFF0000u) * v_inv);
-                    }
                     const uint32_t x0 = __byte_perm(w[0][c2], w[1][c2], 0x5410), x1 = __byte_perm(w[0][c2], w[1][c2], 0x7632);
                     const uint32_t y0 = __byte_perm(w[2][c2], w[3][c2], 0x5410), y1 = __byte_perm(w[2][c2], w[3][c2], 0x7632);
                     mma<false>(o[c2 * 4 + 0], codes<0>(x0), codes<0>(x1), codes<0>(y0), codes<0>(y1), b0, b1);
