@@ -2,7 +2,7 @@
 //
 // attend_step: few queries per request.  Rows are the (token, query head) pairs of a KV head, eight at a time; a unit is (request, KV
 // head, eight rows), and its work the tiles of 16 keys that they see.  All tiles of a call form one line, dealt to the CTAs in equal
-// runs; inside a run a warp takes every eighth (or sixth) tile, on its own: it copies the tile's rows into a ring of its own (cp.async, no barrier),
+// runs; inside a run a warp takes every eighth (sixth, twelfth) tile, on its own: it copies the tile's rows into a ring of its own (cp.async, no barrier),
 // multiplies them as they lie and keeps running maxima, sums and outputs in registers.  Scores are keys x dims x queries with
 // the 16 keys as rows of mma.sync (m16n8k16), outputs dims x keys x queries; which dims and keys stand for which
 // row or column of a fragment is free, and chosen so that a lane multiplies whole 16-byte runs of the cache rows.
@@ -73,8 +73,8 @@ template <int HD, int KIND> struct Layout {
     static constexpr int ROW = KIND == K_INT4 ? HD / 2 : HD * 2;                   // bytes of a cache row
     static constexpr int META = KIND == K_INT4 ? HD / 64 * 4 : 0;
     static constexpr int SLOT = A_KEYS * 2 * (ROW + META);
-    static constexpr int WARPS = KIND != K_INT4 && HD == 256 ? 6 : 8;
-    static constexpr int DEPTH = KIND == K_INT4 ? (HD == 256 ? 5 : 8) : (HD == 256 ? 2 : (HD == 128 ? 3 : 6));
+    static constexpr int WARPS = HD == 256 ? (KIND == K_INT4 ? 12 : 6) : 8;
+    static constexpr int DEPTH = KIND == K_INT4 ? (HD == 256 ? 3 : 8) : (HD == 256 ? 2 : (HD == 128 ? 3 : 6));
     static constexpr int JOIN = WARPS * A_ROWS * (HD + 2) * 4;                     // what the warps leave for one another
     static constexpr int RING = WARPS * DEPTH * SLOT > JOIN ? WARPS * DEPTH * SLOT : JOIN;
     static constexpr int REC = 4 + A_ROWS * (HD + 2);                              // floats of a part: header, outputs, maxima, sums
@@ -504,37 +504,65 @@ static __global__ void __launch_bounds__(Layout<HD, KIND>::WARPS * 32, 1) attend
     grid_release();
 }
 
-// Block c adds up the unit that starts in CTA c and does not end there: its part, then one part of every following CTA until
-// the one that ends it.
+// Block (c, y) adds up 64 dims of the unit that starts in CTA c and does not end there: its part, then one part of every following CTA until the one that
+// ends it.  Maxima and sums of all parts first, side by side, so that nothing is carried from part to part: a single long context is in as many parts
+// as there are CTAs (30000 positions of one request, one part after the other: 93 us a call; so 25).
+constexpr int J_GROUPS = 4, J_THREADS = J_GROUPS * 256, J_PARTS = 256;
 template <int HD>
-static __global__ void __launch_bounds__(256) attend_join(const __grid_constant__ AttendArgs A, int ctas) {
+static __global__ void __launch_bounds__(J_THREADS) attend_join(const __grid_constant__ AttendArgs A, int ctas) {
     constexpr int REC = 4 + A_ROWS * (HD + 2);
+    __shared__ float weight[J_PARTS][A_ROWS];
+    __shared__ float2 sums[J_GROUPS - 1][256];
+    __shared__ int last_s;
     grid_wait();
-    const int c = blockIdx.x;
+    const int c = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const float* first = A.part + ((size_t)c * 2 + 1) * REC;
     const int4 head = *reinterpret_cast<const int4*>(first);
     if (!head.x || (head.x & 2)) return;
-    int last = c + 1;
-    while (last < ctas && !(*reinterpret_cast<const int*>(A.part + (size_t)last * 2 * REC) & 2)) last++;
-    const Span s = span_of(A, head.y);
-    const int row0 = head.w, rows = min(A_ROWS, s.count * A.per - row0);
-    for (int i = threadIdx.x; i < rows * HD / 2; i += 256) {
-        const int n = i / (HD / 2), d = (i - n * (HD / 2)) * 2;
-        float m = -INFINITY, l = 0.f, a = 0.f, b = 0.f;
-        for (int x = c; x <= last && x < ctas; x++) {
-            const float* p = x == c ? first : A.part + (size_t)x * 2 * REC;
-            const float pm = p[4 + A_ROWS * HD + n], pl = p[4 + A_ROWS * HD + A_ROWS + n];
-            if (pm == -INFINITY) continue;
-            const float2 v = *reinterpret_cast<const float2*>(p + 4 + n * HD + d);
-            const float next = fmaxf(m, pm), f = m == -INFINITY ? 0.f : exp2f(m - next), e = exp2f(pm - next);
-            m = next;
-            l = fmaf(l, f, pl * e), a = fmaf(a, f, v.x * e), b = fmaf(b, f, v.y * e);
+    if (tid == 0) last_s = ctas - 1;
+    __syncthreads();
+    for (int x = c + 1 + tid; x < ctas; x += J_THREADS)
+        if (*reinterpret_cast<const int*>(A.part + (size_t)x * 2 * REC) & 2) atomicMin(&last_s, x);
+    __syncthreads();
+    const int parts = last_s - c + 1;
+    auto part = [&](int i) { return i == 0 ? first : A.part + (size_t)(c + i) * 2 * REC; };
+    for (int i = tid; i < parts * A_ROWS; i += J_THREADS) weight[i / A_ROWS][i % A_ROWS] = part(i / A_ROWS)[4 + A_ROWS * HD + i % A_ROWS];
+    __syncthreads();
+    if (warp < A_ROWS) {
+        float m = -INFINITY, l = 0.f;
+        for (int i = lane; i < parts; i += 32) m = fmaxf(m, weight[i][warp]);
+#pragma unroll
+        for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, d));
+        for (int i = lane; i < parts; i += 32) {
+            const float pm = weight[i][warp], f = pm == -INFINITY ? 0.f : exp2_fast(pm - m);
+            if (f > 0.f) l = fmaf(f, part(i)[4 + A_ROWS * HD + A_ROWS + warp], l);
+            weight[i][warp] = f;
         }
-        const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-        const int token = (row0 + n) / A.per, h = row0 + n - token * A.per;
-        uint16_t* dst = reinterpret_cast<uint16_t*>(A.out) + (s.first + token) * A.out_tok + (long long)(head.z * A.per + h) * A.out_head + d;
-        *reinterpret_cast<uint32_t*>(dst) = A.q_f16 ? pack_half(a * inv, b * inv) : pack_bf(a * inv, b * inv);
+#pragma unroll
+        for (int d = 16; d; d >>= 1) l += __shfl_xor_sync(~0u, l, d);
+        const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);                // (a sum that is NaN stays one)
+        for (int i = lane; i < parts; i += 32) weight[i][warp] *= inv;
     }
+    __syncthreads();
+    const Span s = span_of(A, head.y);
+    const int row0 = head.w, rows = min(A_ROWS, s.count * A.per - row0), group = tid >> 8, at = tid & 255, n = at >> 5, d = blockIdx.y * 64 + (at & 31) * 2;
+    float2 sum = make_float2(0.f, 0.f);
+    if (n < rows) {
+#pragma unroll 8
+        for (int i = group; i < parts; i += J_GROUPS) {
+            const float w = weight[i][n];
+            const float2 v = *reinterpret_cast<const float2*>(part(i) + 4 + n * HD + d);
+            if (w != 0.f) sum.x = fmaf(w, v.x, sum.x), sum.y = fmaf(w, v.y, sum.y);
+        }
+    }
+    if (group) sums[group - 1][at] = sum;
+    __syncthreads();
+    if (group || n >= rows) return;
+#pragma unroll
+    for (int g = 0; g < J_GROUPS - 1; g++) sum.x += sums[g][at].x, sum.y += sums[g][at].y;
+    const int token = (row0 + n) / A.per, h = row0 + n - token * A.per;
+    uint16_t* dst = reinterpret_cast<uint16_t*>(A.out) + (s.first + token) * A.out_tok + (long long)(head.z * A.per + h) * A.out_head + d;
+    *reinterpret_cast<uint32_t*>(dst) = A.q_f16 ? pack_half(sum.x, sum.y) : pack_bf(sum.x, sum.y);
 }
 
 static int sm_count(int device) {
@@ -546,9 +574,10 @@ template <int HD, int KIND>
 static int launch_step(const AttendArgs& A, int sms, cudaStream_t st) {
     using L = Layout<HD, KIND>;
     const size_t smem = L::RING + (size_t)(A.R + 1) * 8;
+    if (sms > J_PARTS) return vfail(MK_ERR_UNSUPPORTED, "mk_attend: %d SMs", sms);
     MKV_CUDA(cudaFuncSetAttribute(attend_step<HD, KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     MKV_CUDA(launch(attend_step<HD, KIND>, dim3(sms), L::WARPS * 32, smem, 1, false, st, A));
-    MKV_CUDA(launch(attend_join<HD>, dim3(sms), 256, 0, 1, true, st, A, sms));
+    MKV_CUDA(launch(attend_join<HD>, dim3(sms, HD / 64), J_THREADS, 0, 1, true, st, A, sms));
     return MK_OK;
 }
 template <int HD>
