@@ -194,25 +194,34 @@ struct HeadsArgs {
 
 __device__ __forceinline__ float2 unpack(uint32_t w, __nv_bfloat16) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u)); }
 __device__ __forceinline__ float2 unpack(uint32_t w, __half) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
-// V neighbouring elements
-template <int V> __device__ __forceinline__ void load_piece(float* x, const float* p) {
-    if constexpr (V == 4) {
-        const float4 a = *reinterpret_cast<const float4*>(p);
-        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w;
-    } else {
-        const float2 a = *reinterpret_cast<const float2*>(p);
-        x[0] = a.x, x[1] = a.y;
+// V neighbouring elements, as they lie and as values.
+template <class T, int V> struct Piece {
+    static constexpr int WORDS = V * sizeof(T) / 4;
+    uint32_t w[WORDS];
+    __device__ __forceinline__ void load(const T* p) {
+        if constexpr (WORDS == 4) *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(p);
+        else if constexpr (WORDS == 2) *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(p);
+        else w[0] = *reinterpret_cast<const uint32_t*>(p);
     }
-}
-template <int V, class T> __device__ __forceinline__ void load_piece(float* x, const T* p) {
-    uint32_t w[V / 2];
-    if constexpr (V == 4) *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(p);
-    else w[0] = *reinterpret_cast<const uint32_t*>(p);
+    __device__ __forceinline__ void zero() {
 #pragma unroll
-    for (int i = 0; i < V / 2; i++) {
-        const float2 v = unpack(w[i], T());
-        x[2 * i] = v.x, x[2 * i + 1] = v.y;
+        for (int i = 0; i < WORDS; i++) w[i] = 0u;
     }
+    __device__ __forceinline__ void values(float* x) const {
+#pragma unroll
+        for (int i = 0; i < WORDS; i++) {
+            if constexpr (sizeof(T) == 4) x[i] = __uint_as_float(w[i]);
+            else {
+                const float2 v = unpack(w[i], T());
+                x[2 * i] = v.x, x[2 * i + 1] = v.y;
+            }
+        }
+    }
+};
+template <int V> __device__ __forceinline__ void load_piece(float* x, const float* p) {
+    Piece<float, V> v;
+    v.load(p);
+    v.values(x);
 }
 template <int V> __device__ __forceinline__ void store_piece(uint16_t* p, const float* x, bool f16) {
     uint32_t w[V / 2];
@@ -280,35 +289,57 @@ static __global__ void __launch_bounds__(256) heads_kernel(const __grid_constant
     int from[PIECES];
     bool other[PIECES];
     const int half = A.rot / 2;
+    // (a piece's angles are neighbours; the tables' rows allow whole loads where a row is whole pieces)
+    const bool wide = A.pairs % V == 0 && !A.interleaved;
 #pragma unroll
-    for (int i = 0; i < N; i++) {
-        const int d = dim_of(i), pair = A.interleaved ? d >> 1 : (d < half ? d : d - half);
-        const bool turned = A.cos && live && d < A.rot && pair < A.pairs;
-        turns |= (uint32_t)turned << i;
-        c[i] = turned ? __ldg(A.cos + (size_t)pos * A.pairs + pair) : 1.f;
-        s[i] = turned ? __ldg(A.sin + (size_t)pos * A.pairs + pair) : 0.f;
-        if (A.interleaved ? !(d & 1) : d < half) s[i] = -s[i];
-        if (i % V == 0) {
-            const int p = d >= A.rot ? d : (d < half ? d + half : d - half);         // (half is a multiple of V)
-            from[i / V] = (p & 127) / V;
-            other[i / V] = p / 128 != i / V;
+    for (int p = 0; p < PIECES; p++) {
+        const int d0 = dim_of(p * V), first = A.interleaved ? d0 >> 1 : (d0 < half ? d0 : d0 - half);      // (half is a multiple of V)
+#pragma unroll
+        for (int i = 0; i < V; i++) c[p * V + i] = 1.f, s[p * V + i] = 0.f;
+        if (A.cos && live && d0 < A.rot) {
+            const size_t row = (size_t)pos * A.pairs;
+            if (wide) {
+                if (first < A.pairs) {
+                    load_piece<V>(c + p * V, A.cos + row + first);
+                    load_piece<V>(s + p * V, A.sin + row + first);
+                    turns |= ((1u << V) - 1) << (p * V);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < V; i++) {
+                    const int pair = A.interleaved ? (d0 + i) >> 1 : first + i;
+                    if (pair < A.pairs) c[p * V + i] = __ldg(A.cos + row + pair), s[p * V + i] = __ldg(A.sin + row + pair), turns |= 1u << (p * V + i);
+                }
+            }
         }
+#pragma unroll
+        for (int i = 0; i < V; i++)
+            if (A.interleaved ? !(i & 1) : d0 < half) s[p * V + i] = -s[p * V + i];
+        const int partner = d0 >= A.rot ? d0 : (d0 < half ? d0 + half : d0 - half);
+        from[p] = (partner & 127) / V;
+        other[p] = partner / 128 != p;
     }
     const bool near = PIECES == 1 || half <= 64;                      // partners in the same piece
     const int total = A.nq + (A.cache_type >= 0 ? 2 : 1) * A.nkv, stride = 8 * gridDim.y;
-    for (int h = blockIdx.y * 8 + warp; h < total; h += stride) {
-        const int kind = h < A.nq ? 0 : (h < A.nq + A.nkv ? 1 : 2), head = kind == 0 ? h : (kind == 1 ? h - A.nq : h - A.nq - A.nkv);
-        const T* src = kind == 0 ? reinterpret_cast<const T*>(A.q) + (long long)t * A.q_tok + head * A.q_head
-                                 : (kind == 1 ? reinterpret_cast<const T*>(A.k) + (long long)t * A.k_tok + head * A.k_head
-                                              : reinterpret_cast<const T*>(A.v) + (long long)t * A.v_tok + head * A.v_head);
-        float x[N];
+    Piece<T, V> next[PIECES];
+    auto fetch = [&](int h) {
+        const T* src = h < A.nq ? reinterpret_cast<const T*>(A.q) + (long long)t * A.q_tok + h * A.q_head
+                                : (h < A.nq + A.nkv ? reinterpret_cast<const T*>(A.k) + (long long)t * A.k_tok + (h - A.nq) * A.k_head
+                                                    : reinterpret_cast<const T*>(A.v) + (long long)t * A.v_tok + (h - A.nq - A.nkv) * A.v_head);
 #pragma unroll
         for (int p = 0; p < PIECES; p++) {
-            if (live) load_piece<V>(x + p * V, src + dim_of(p * V));
-            else
-#pragma unroll
-                for (int i = 0; i < V; i++) x[p * V + i] = 0.f;
+            if (live) next[p].load(src + dim_of(p * V));
+            else next[p].zero();
         }
+    };
+    int h = blockIdx.y * 8 + warp;
+    if (h < total) fetch(h);
+    for (; h < total; h += stride) {
+        const int kind = h < A.nq ? 0 : (h < A.nq + A.nkv ? 1 : 2), head = kind == 0 ? h : (kind == 1 ? h - A.nq : h - A.nq - A.nkv);
+        float x[N];
+#pragma unroll
+        for (int p = 0; p < PIECES; p++) next[p].values(x + p * V);
+        if (h + stride < total) fetch(h + stride);                    // the next head is on its way while this one is turned
         const float* w = kind == 0 ? A.q_norm : (kind == 1 ? A.k_norm : nullptr);
         if (w || (kind == 2 && A.v_norm)) {
             float sq[V];

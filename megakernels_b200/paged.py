@@ -71,7 +71,7 @@ class PagePool:
         serve.whole("lengths", lengths, self.requests)
         serve.whole("new", new, self.requests)
         serve.on_gpu(self.table, lengths, new)
-        code = self.lib.mk_page_plan(serve.pack_plan(lengths.data_ptr(), new.data_ptr(), *self._args), serve.raw_stream(self.device, stream))
+        code = self.lib.mk_page_plan(serve.pack_plan(lengths.data_ptr(), new.data_ptr(), *self._args), serve.raw_stream(self.device.index, stream))
         if code:
             _lib.check(code)
         return self._plan
@@ -128,7 +128,7 @@ class Cache:
             raise ValueError(f"{self.page} tokens per page (a power of two, 16 or more)")
         if not 1 <= self.pages * self.page < 2 ** 31 or self.kv_heads < 1:
             raise ValueError(f"{self.pages} pages of {self.page} tokens, {self.kv_heads} heads (slots have 32 bits)")
-        self.device = serve.on_gpu(k, v, ks, vs)
+        self.device = torch.device("cuda", serve.on_gpu(k, v, ks, vs))
         if self.int4:
             shape = (self.pages, self.kv_heads, self.page, self.head_dim // serve.GROUP, 2)
             if k.dtype != torch.uint8 or not (k.is_contiguous() and v.is_contiguous()):
@@ -154,10 +154,10 @@ class Cache:
         n = slots.numel()
         serve.whole("slots", slots, n)
         serve.on_gpu(self.k, slots)
-        out = serve.empty((2, n, self.kv_heads, self.head_dim), torch.float32 if self.int4 else self.dtype, self.device, stream)
+        out = serve.empty((2, n, self.kv_heads, self.head_dim), torch.float32 if self.int4 else self.dtype, self.device.index, stream)
         k, v = out[0], out[1]
         if n:
-            code = serve.lib().mk_cache_rows(ctypes.byref(self.desc), slots.data_ptr(), n, k.data_ptr(), v.data_ptr(), self.device.index, serve.raw_stream(self.device, stream))
+            code = serve.lib().mk_cache_rows(ctypes.byref(self.desc), slots.data_ptr(), n, k.data_ptr(), v.data_ptr(), self.device.index, serve.raw_stream(self.device.index, stream))
             if code:
                 _lib.check(code)
         return k, v
@@ -214,7 +214,7 @@ def _heads(q, k, v, positions, slots, cache, rope, rot, q_norm, k_norm, norm_off
         at = lambda t: t.data_ptr() if t is not None else 0                            # noqa: E731
         a = serve.pack_heads(q.data_ptr(), k.data_ptr(), at(v), out.data_ptr(), at(k_out), positions.data_ptr(), at(slots), at(q_norm), at(k_norm), at(cos), at(sin),
                              *q.stride()[:2], *k.stride()[:2], *(v.stride()[:2] if v is not None else (0, 0)), *(cache._args if cache is not None else serve.NO_CACHE), eps, norm_offset,
-                             T, nq, nkv, dim, serve.TYPES[q.dtype], serve.TYPES[dtype], rot or 0, angles, longest, bool(interleaved), bool(v_norm), device.index)
+                             T, nq, nkv, dim, serve.TYPES[q.dtype], serve.TYPES[dtype], rot or 0, angles, longest, bool(interleaved), bool(v_norm), device)
         code = serve.lib().mk_heads(a, serve.raw_stream(device, stream))
         if code:
             _lib.check(code)
@@ -241,21 +241,23 @@ def enter(q, k, v, positions, slots, cache, rope=None, rot=None, q_norm=None, k_
     return _heads(q, k, v, positions, slots, cache, rope, rot, q_norm, k_norm, norm_offset, eps, interleaved, v_norm, dtype, out, stream)[0]
 
 
-_status = {}
+_status, _bytes = {}, {}
 
 
-def _status_of(device):
-    if device not in _status:
-        _status[device] = torch.zeros(4, dtype=torch.int32, device=device)
-    return _status[device]
+def _status_of(index):
+    """Where the calls on a device leave word of a wait that ran out."""
+    st = _status.get(index)
+    if st is None:
+        st = _status[index] = torch.zeros(4, dtype=torch.int32, device=index)
+    return st
 
 
 def check(device=None):
     """Synchronise and raise if a device-side wait ran out in any call so far on this device (default: the current one)."""
-    device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
-    st = _status_of(device).tolist()
+    index = torch.cuda.current_device() if device is None else torch.device(device).index
+    st = _status_of(index).tolist()
     if st[0] != 0:
-        _status_of(device).zero_()
+        _status_of(index).zero_()
         raise _lib.MkError(_lib.MK_ERR_TIMEOUT, f"a device-side wait ran out (site {st[1]}, CTA {st[2]}, thread {st[3]})")
 
 
@@ -304,11 +306,14 @@ def attend(q, cache, table, context, starts=None, max_new=None, scale=None, wind
     if not _rows_ok(q, 16):
         raise ValueError("q: neighbouring dims, rows on 16-byte boundaries")
     fixed = (*q.stride()[:2], *out.stride()[:2], table.stride(0), *cache._args, 0, dim ** -0.5 if scale is None else scale, serve.TYPES[q.dtype], R, T, nq, pages, min(max_new, T),
-             min(window, 2 ** 31 - 1), min(sinks, 2 ** 31 - 1), device.index)
+             min(window, 2 ** 31 - 1), min(sinks, 2 ** 31 - 1), device)
     front = (q.data_ptr(), out.data_ptr(), table.data_ptr(), context.data_ptr(), starts.data_ptr() if starts is not None else 0)
-    need = lib.mk_attend_bytes(serve.pack_attend(*front, 0, 0, *fixed))
-    if need < 0:
-        _lib.check(int(need))
+    need = _bytes.get((device, dim))                               # it depends on nothing else
+    if need is None:
+        need = lib.mk_attend_bytes(serve.pack_attend(*front, 0, 0, *fixed))
+        if need < 0:
+            _lib.check(int(need))
+        _bytes[device, dim] = need
     work = serve.empty((need,), torch.uint8, device, stream)
     code = lib.mk_attend(serve.pack_attend(*front, work.data_ptr(), _status_of(device).data_ptr(), *fixed), serve.raw_stream(device, stream))
     if code:

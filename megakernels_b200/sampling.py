@@ -64,10 +64,11 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, stream=Non
                 with torch.cuda.stream(stream):
                     have.fill_(asked)
     out = serve.empty((3, rows), torch.int32, device, stream)
-    ids, logprobs, kept = out[0], out[1].view(torch.float32), out[2]
+    ids, logprobs, kept = out.unbind(0)
+    logprobs = logprobs.view(torch.float32)
     if rows:
         a = serve.pack_sample(logits.data_ptr(), u.data_ptr(), t.data_ptr(), p.data_ptr(), m.data_ptr(), k.data_ptr(), ids.data_ptr(), logprobs.data_ptr(), kept.data_ptr(),
-                              logits.stride(0), rows, vocab, serve.TYPES[logits.dtype], device.index)
+                              logits.stride(0), rows, vocab, serve.TYPES[logits.dtype], device)
         code = lib.mk_sample(a, serve.raw_stream(device, stream))
         if code:
             _lib.check(code)

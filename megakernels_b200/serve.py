@@ -84,17 +84,18 @@ NO_CACHE = (0,) * 13
 
 
 def on_gpu(*tensors):
-    """Refuses tensors (None aside) that are not on one CUDA device; returns it."""
-    first = None
+    """Refuses tensors (None aside) that are not on one CUDA device; returns its index."""
+    first = -1
     for t in tensors:
         if t is None:
             continue
-        if first is None:
-            if not t.is_cuda:
+        at = t.get_device()
+        if at != first or at < 0:
+            if at < 0:
                 raise ValueError(f"a tensor on {t.device}: the serving operators have no CPU path")
-            first = t.device
-        elif t.device != first:
-            raise ValueError(f"tensors on {first} and {t.device}")
+            if first >= 0:
+                raise ValueError(f"tensors on cuda:{first} and {t.device}")
+            first = at
     return first
 
 
@@ -104,14 +105,14 @@ def whole(name, t, *shape):
         raise ValueError(f"{name}: contiguous int32 {list(shape)}, got {t.dtype} {list(t.shape)}")
 
 
-def raw_stream(device, stream):
-    """The stream a call goes to, as the C ABI takes it."""
-    return stream.cuda_stream if stream is not None else torch._C._cuda_getCurrentRawStream(device.index)
+def raw_stream(index, stream):
+    """The stream a call on the device of this index goes to, as the C ABI takes it."""
+    return stream.cuda_stream if stream is not None else torch._C._cuda_getCurrentRawStream(index)
 
 
-def empty(shape, dtype, device, stream):
+def empty(shape, dtype, index, stream):
     """Memory of PyTorch's allocator that belongs to the stream of the call."""
     if stream is None:
-        return torch.empty(shape, dtype=dtype, device=device)
+        return torch.empty(shape, dtype=dtype, device=index)
     with torch.cuda.stream(stream):
-        return torch.empty(shape, dtype=dtype, device=device)
+        return torch.empty(shape, dtype=dtype, device=index)
