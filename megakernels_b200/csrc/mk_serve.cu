@@ -255,11 +255,15 @@ __device__ __forceinline__ void store_codes(uint8_t* row, uint32_t* scales, cons
     const __nv_bfloat16 low = __float2bfloat16_rd(lo);
     const float base = __bfloat162float(low);
     const __nv_bfloat16 step = __float2bfloat16_ru(__fmul_rn(__fadd_rn(hi, -base), 1.f / 15.f));
-    const float s = __bfloat162float(step);
+    const float s = __bfloat162float(step), inv = __frcp_rn(s);
     uint32_t word = 0;
 #pragma unroll
     for (int i = 0; i < V; i++) {
-        const float c = s > 0.f ? rintf(__fdiv_rn(__fadd_rn(x[i], -base), s)) : 0.f;
+        // the quotient rounded as a division would round it, at the price of a product: only one that lies near a half can fall the other way
+        const float a = __fadd_rn(x[i], -base), q = a * inv;
+        float c = rintf(q);
+        if (fabsf(q - c) > 0.49999f) c = rintf(__fdiv_rn(a, s));
+        if (!(s > 0.f)) c = 0.f;
         word |= (uint32_t)(c >= 0.f ? fminf(c, 15.f) : 0.f) << (4 * i);      // (a NaN compares false)
     }
     constexpr int SHARE = 8 / V;                                      // lanes of a word
@@ -272,10 +276,22 @@ __device__ __forceinline__ void store_codes(uint8_t* row, uint32_t* scales, cons
 }
 
 template <class T, int N>
-static __global__ void __launch_bounds__(256) heads_kernel(const __grid_constant__ HeadsArgs A) {
+static __global__ void __launch_bounds__(256, 4) heads_kernel(const __grid_constant__ HeadsArgs A) {
     constexpr int D = 32 * N, V = N < 4 ? N : 4, PIECES = N / V;
     const int t = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     auto dim_of = [&](int i) { return i / V * 128 + lane * V + i % V; };
+    const int total = A.nq + (A.cache_type >= 0 ? 2 : 1) * A.nkv, stride = 8 * gridDim.y;
+    // (the first head's row does not depend on where the token goes: it is asked for first)
+    Piece<T, V> next[PIECES];
+    auto fetch = [&](int h) {
+        const T* src = h < A.nq ? reinterpret_cast<const T*>(A.q) + (long long)t * A.q_tok + h * A.q_head
+                                : (h < A.nq + A.nkv ? reinterpret_cast<const T*>(A.k) + (long long)t * A.k_tok + (h - A.nq) * A.k_head
+                                                    : reinterpret_cast<const T*>(A.v) + (long long)t * A.v_tok + (h - A.nq - A.nkv) * A.v_head);
+#pragma unroll
+        for (int p = 0; p < PIECES; p++) next[p].load(src + dim_of(p * V));
+    };
+    int h = blockIdx.y * 8 + warp;
+    if (h < total) fetch(h);
     const int pos = A.positions[t];
     bool live = A.cos ? pos >= 0 && pos < A.max_position : true;
     int slot = 0;
@@ -320,25 +336,14 @@ static __global__ void __launch_bounds__(256) heads_kernel(const __grid_constant
         other[p] = partner / 128 != p;
     }
     const bool near = PIECES == 1 || half <= 64;                      // partners in the same piece
-    const int total = A.nq + (A.cache_type >= 0 ? 2 : 1) * A.nkv, stride = 8 * gridDim.y;
-    Piece<T, V> next[PIECES];
-    auto fetch = [&](int h) {
-        const T* src = h < A.nq ? reinterpret_cast<const T*>(A.q) + (long long)t * A.q_tok + h * A.q_head
-                                : (h < A.nq + A.nkv ? reinterpret_cast<const T*>(A.k) + (long long)t * A.k_tok + (h - A.nq) * A.k_head
-                                                    : reinterpret_cast<const T*>(A.v) + (long long)t * A.v_tok + (h - A.nq - A.nkv) * A.v_head);
-#pragma unroll
-        for (int p = 0; p < PIECES; p++) {
-            if (live) next[p].load(src + dim_of(p * V));
-            else next[p].zero();
-        }
-    };
-    int h = blockIdx.y * 8 + warp;
-    if (h < total) fetch(h);
     for (; h < total; h += stride) {
         const int kind = h < A.nq ? 0 : (h < A.nq + A.nkv ? 1 : 2), head = kind == 0 ? h : (kind == 1 ? h - A.nq : h - A.nq - A.nkv);
         float x[N];
 #pragma unroll
-        for (int p = 0; p < PIECES; p++) next[p].values(x + p * V);
+        for (int p = 0; p < PIECES; p++) {
+            if (!live) next[p].zero();
+            next[p].values(x + p * V);
+        }
         if (h + stride < total) fetch(h + stride);                    // the next head is on its way while this one is turned
         const float* w = kind == 0 ? A.q_norm : (kind == 1 ? A.k_norm : nullptr);
         if (w || (kind == 2 && A.v_norm)) {
@@ -360,21 +365,30 @@ static __global__ void __launch_bounds__(256) heads_kernel(const __grid_constant
             }
         }
         if (kind < 2 && A.cos) {
-            float y[N];
+            float z[N];                                               // the partners
+            if (A.interleaved) {
 #pragma unroll
-            for (int i = 0; i < N; i++) {
-                float z;
-                if (A.interleaved) z = x[i ^ 1];
-                else if (near) z = __shfl_sync(~0u, x[i], from[i / V]);
-                else if (half == 128) z = x[(i + V) % N];
-                else {
+                for (int i = 0; i < N; i++) z[i] = x[i ^ 1];
+            } else if (PIECES == 2 && half == 128) {
+#pragma unroll
+                for (int i = 0; i < N; i++) z[i] = x[(i + V) % N];
+            } else if (near) {
+#pragma unroll
+                for (int i = 0; i < V; i++) z[i] = __shfl_sync(~0u, x[i], from[0]);
+#pragma unroll
+                for (int i = V; i < N; i++) z[i] = 0.f;               // (these dims are not turned: near ends at the first piece)
+            } else {
+#pragma unroll
+                for (int i = 0; i < N; i++) {
                     const float a = __shfl_sync(~0u, x[i], from[i / V]), b = __shfl_sync(~0u, x[(i + V) % N], from[i / V]);
-                    z = other[i / V] ? b : a;
+                    z[i] = other[i / V] ? b : a;
                 }
-                y[i] = turns >> i & 1 ? x[i] * c[i] + z * s[i] : x[i];
             }
 #pragma unroll
-            for (int i = 0; i < N; i++) x[i] = y[i];
+            for (int i = 0; i < N; i++) {
+                const float y = x[i] * c[i] + z[i] * s[i];
+                x[i] = turns >> i & 1 ? y : x[i];
+            }
         }
         if (kind == 0 || A.cache_type < 0) {
             uint16_t* out = reinterpret_cast<uint16_t*>(kind == 0 ? A.q_out : A.k_out) + ((size_t)t * (kind == 0 ? A.nq : A.nkv) + head) * D;
