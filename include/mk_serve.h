@@ -66,7 +66,7 @@ typedef struct {
  * normed without a weight (v_norm).  With a cache, k and v of token t enter slot slots[t]; a token whose slot is outside
  * the cache, or whose position is outside the tables, is padding: zeros in q_out (and k_out), nothing written. */
 typedef struct {
-    uint64_t q, k, v;                /* [tokens][heads][head_dim] of `source`; v 0 without a cache             */
+    uint64_t q, k, v;                /* [tokens][heads][head_dim] of `source`; v 0 without a cache; q 0 with no query heads */
     uint64_t q_out, k_out;           /* [tokens][heads][head_dim] of `type`, contiguous; k_out only without a cache */
     uint64_t positions, slots;       /* i32[tokens]; slots only with a cache                                   */
     uint64_t q_norm, k_norm;         /* fp32 [head_dim] or 0: no norm                                          */

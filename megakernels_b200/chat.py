@@ -24,8 +24,8 @@ class TextStream:
         return fresh
 
 
-def repl(session, system=None, temperature=0.7, max_new_tokens=2048, think=False, inp=input, out=sys.stdout):
-    """The read-reply loop.  `inp` / `out` are injectable for tests."""
+def repl(session, system=None, temperature=0.7, max_new_tokens=2048, think=False, inp=input, out=sys.stdout, **filters):
+    """The read-reply loop.  `inp` / `out` are injectable for tests; `filters`: top_k, top_p, min_p."""
     base = [{"role": "system", "content": system}] if system else []
     messages, show_stats = list(base), True
     while True:
@@ -47,7 +47,7 @@ def repl(session, system=None, temperature=0.7, max_new_tokens=2048, think=False
             continue
         messages.append({"role": "user", "content": line})
         text, stream = "", TextStream(session.tok)
-        for t in session.chat(messages, enable_thinking=think, temperature=temperature, max_new_tokens=max_new_tokens):
+        for t in session.chat(messages, enable_thinking=think, temperature=temperature, max_new_tokens=max_new_tokens, **filters):
             piece = stream.push(t)
             text += piece
             out.write(piece)
@@ -63,6 +63,9 @@ def main():
     ap = argparse.ArgumentParser(description=__doc__, formatter_class=argparse.RawDescriptionHelpFormatter)
     ap.add_argument("--model", required=True, help="local snapshot directory (this library never downloads)")
     ap.add_argument("--temperature", type=float, default=0.7, help="0 = greedy")
+    ap.add_argument("--top-k", type=int, default=0, help="0 = all")
+    ap.add_argument("--top-p", type=float, default=1.0)
+    ap.add_argument("--min-p", type=float, default=0.0)
     ap.add_argument("--max-new-tokens", type=int, default=2048)
     ap.add_argument("--system", default=None)
     ap.add_argument("--think", action="store_true")
@@ -73,7 +76,7 @@ def main():
     from .session import ChatSession
     session = ChatSession.from_snapshot(args.model, max_seq=args.max_seq, quant=args.quant, spec=not args.no_spec)
     print("ready. /reset, /stats, /quit", file=sys.stderr)
-    repl(session, args.system, args.temperature, args.max_new_tokens, args.think)
+    repl(session, args.system, args.temperature, args.max_new_tokens, args.think, top_k=args.top_k, top_p=args.top_p, min_p=args.min_p)
 
 
 if __name__ == "__main__":

@@ -519,7 +519,7 @@ extern "C" int mk_heads(const mk_heads_args* a, void* stream) {
     if (a->source < 0 || a->source > MKV_F32) return vfail(MK_ERR_BADARG, "mk_heads: source type %d", a->source);
     if (a->type != MKV_BF16 && a->type != MKV_F16) return vfail(MK_ERR_BADARG, "mk_heads: output type %d", a->type);
     const bool cached = a->cache.k != 0;
-    if (!a->q || !a->k || !a->q_out || !a->positions || (cached && (!a->v || !a->slots)) || (!cached && !a->k_out)) return vfail(MK_ERR_BADARG, "mk_heads: a buffer is missing");
+    if ((a->q_heads && (!a->q || !a->q_out)) || !a->k || !a->positions || (cached && (!a->v || !a->slots)) || (!cached && !a->k_out)) return vfail(MK_ERR_BADARG, "mk_heads: a buffer is missing");
     if (cached) {
         if (const char* why = bad_cache(a->cache)) return vfail(MK_ERR_BADARG, "mk_heads: %s", why);
         if (a->cache.head_dim != D || a->cache.kv_heads != a->kv_heads) return vfail(MK_ERR_BADARG, "mk_heads: cache of %d heads of %d", a->cache.kv_heads, a->cache.head_dim);

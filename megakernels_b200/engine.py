@@ -25,6 +25,7 @@ import torch
 
 from . import _lib
 from . import mtp as mtp_mod
+from . import sampling
 from .config import Config
 from .pack import as_bytes, pack_down_cols, pack_out_cols, pack_rows
 from .quant import is_gemv_weight, quantize_int8_rows, roundtrip_int8_rows
@@ -712,11 +713,25 @@ class Megakernel:
             self.last_logits = bufs["logits_out"][:cycles_run]
         return ids, next_draft
 
-    def generate(self, prompt_ids, max_new_tokens=256, temperature=0.0, seed=0, stop_ids=(), chunk=16, spec=False):
+    def generate(self, prompt_ids, max_new_tokens=256, temperature=0.0, seed=0, stop_ids=(), chunk=16, spec=False, top_k=0, top_p=1.0, min_p=0.0):
         """Generator over the ids the model produces after `prompt_ids` (`qwen_mk/engine.py:307-327`).  The engine's
         state stops right behind the last token it was fed, and `self.pending` keeps the one produced id that has not
-        been fed yet, so a conversation continues by passing the next prompt."""
+        been fed yet, so a conversation continues by passing the next prompt.
+
+        With top_k, top_p or min_p (and a temperature) every token is chosen from the step's logits by `sampling.sample`, its uniform
+        numbers drawn from `seed`: a launch of the engine, one of the choice and a read per token, and no speculative cycles."""
+        sampling.check_settings(top_k=top_k, top_p=top_p, min_p=min_p)
         pending = self.prefill(prompt_ids)
+        if temperature > 0 and (top_k > 0 or top_p < 1 or min_p > 0):
+            u = torch.rand(max(max_new_tokens, 1), generator=torch.Generator(device=self.device).manual_seed(seed), device=self.device)
+            for i in range(max_new_tokens):
+                _, logits = self.run([pending], n_generate=1, return_logits=True)
+                pending = int(sampling.sample(logits[-1:], u[i: i + 1], temperature, top_k, top_p, min_p).ids)
+                yield pending
+                if pending in stop_ids:
+                    return
+            self.pending = pending
+            return
         guess = pending            # the first cycle has no draft yet: whatever is offered can only cost that cycle
         left = max_new_tokens
         while left > 0:

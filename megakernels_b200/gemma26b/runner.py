@@ -19,6 +19,7 @@ import torch
 
 from ..qwen27b.runner import KV_BLOCK, attn_chunk
 from ..stage import desc as D
+from ..stage.kv import SequenceCalls, SharedPages
 from ..stage.runtime import Program, Runtime
 from .pack import Packed
 
@@ -32,8 +33,8 @@ def rope_table(theta, head_dim, pairs, maxlen, device):
     return ang.cos().float().to(device).contiguous(), ang.sin().float().to(device).contiguous()
 
 
-class Engine:
-    def __init__(self, PK: Packed, M: int, maxlen: int = 4096, layers=None, device="cuda", lm_head: bool = True, spin_limit_ms=2000):
+class Engine(SequenceCalls):
+    def __init__(self, PK: Packed, M: int, maxlen: int = 4096, layers=None, device="cuda", lm_head: bool = True, spin_limit_ms=2000, kv_pages=None):
         if not 1 <= M <= D.MAX_BATCH:
             raise ValueError(f"M must lie in [1, {D.MAX_BATCH}]")
         if not torch.cuda.is_available():
@@ -66,14 +67,19 @@ class Engine:
         self.logits = z(M, s.vocab)
         self.keys = z(M, grid, dtype=torch.int64)
         g = torch.Generator().manual_seed(0)
-        self.bt = (torch.randperm(M * nb, generator=g) + 1).reshape(M, nb).to(torch.int32).to(dev)
+        pages = M * nb + 1 if kv_pages is None else kv_pages          # shared by the sequences: see `qwen27b.Engine`
+        if kv_pages is not None:
+            self.pages = SharedPages(M, pages, nb, KV_BLOCK, dev)
+            self.bt = self.pages.pool.table
+        else:
+            self.bt = (torch.randperm(M * nb, generator=g) + 1).reshape(M, nb).to(torch.int32).to(dev)
         pr.hold(self.bt)
         n_full = sum(s.is_full(i) for i in range(self.layers))
         n_slide = self.layers - n_full
-        self.ks = z(n_slide, M * nb + 1, s.nkv_s, KV_BLOCK, s.hd_s, dtype=torch.bfloat16)
-        self.vs = z(n_slide, M * nb + 1, s.nkv_s, KV_BLOCK, s.hd_s, dtype=torch.bfloat16)
-        self.kf = z(n_full, M * nb + 1, s.nkv_f, KV_BLOCK, s.hd_f, dtype=torch.bfloat16)
-        self.vf = z(n_full, M * nb + 1, s.nkv_f, KV_BLOCK, s.hd_f, dtype=torch.bfloat16)
+        self.ks = z(n_slide, pages, s.nkv_s, KV_BLOCK, s.hd_s, dtype=torch.bfloat16)
+        self.vs = z(n_slide, pages, s.nkv_s, KV_BLOCK, s.hd_s, dtype=torch.bfloat16)
+        self.kf = z(n_full, pages, s.nkv_f, KV_BLOCK, s.hd_f, dtype=torch.bfloat16)
+        self.vf = z(n_full, pages, s.nkv_f, KV_BLOCK, s.hd_f, dtype=torch.bfloat16)
         tabs = {False: rope_table(s.theta_s, s.hd_s, s.hd_s // 2, self.maxlen, dev), True: rope_table(s.theta_f, s.hd_f, s.rot_f, self.maxlen, dev)}
         for c, sn in tabs.values():
             pr.hold(c), pr.hold(sn)
@@ -166,10 +172,12 @@ class Engine:
     # ------------------------------------------------------------------------------------------------
     def reset(self):
         self.rt.reset()
+        if self.pages is not None:
+            self.pages.reset()
 
     def step(self, tok: torch.Tensor, valid=None, stream=None):
         self.rt.tok[: self.M].copy_(tok.to(device=self.device, dtype=torch.int32))
-        self.rt.launch(1, stream=stream, row_valid=self._rows(valid))
+        self._advance(self._rows(valid), stream)
         return self.logits
 
     def _rows(self, valid):
@@ -182,19 +190,21 @@ class Engine:
         self.rowv[: self.M].copy_(torch.as_tensor(valid).to(device=self.device, dtype=torch.int32))
         return self.rowv
 
-    def generate(self, tok: torch.Tensor, n_steps: int):
+    def generate(self, tok: torch.Tensor, n_steps: int, temperature=0.0, top_k=0, top_p=1.0, min_p=0.0, seed=0):
         if not self.lm_head:
             raise RuntimeError("generate needs the LM head")
+        if temperature > 0:
+            return self._advance_sampled(tok, n_steps, temperature, top_k, top_p, min_p, seed)
         out = torch.zeros(n_steps, self.M, dtype=torch.int32, device=self.device)
         self.rt.tok[: self.M].copy_(tok.to(device=self.device, dtype=torch.int32))
-        self.rt.launch(n_steps, tokens_out=out)
+        self._advance_greedy(n_steps, out)
         return out
 
     def prefill(self, prompts):
         if len(prompts) != self.M or len({len(p) for p in prompts}) != 1 or not prompts[0]:
             raise ValueError(f"prefill takes {self.M} prompts of one common, non-zero length")
         toks = torch.tensor(prompts, dtype=torch.int32).t().contiguous().to(self.device)
-        self.rt.prefill(toks)
+        self._take_in(toks)
         self._prompt = toks
         return self.logits
 

@@ -148,6 +148,10 @@ class Cache:
         self._args = (at(k), at(v), at(ks), at(vs), *strides, serve.INT4 if self.int4 else serve.TYPES[k.dtype], self.pages, self.kv_heads, self.head_dim, self.page, 0)
         self.desc = serve.CacheDesc(*self._args)
 
+    def put(self, k, v, slots, stream=None):
+        """Keys and values [tokens, kv heads, head dim] (fp32, bf16 or fp16) as they are to `slots` (int32 [tokens]); -1 is padding."""
+        _heads(k[:, :0], k, v, slots, slots, self, None, None, None, None, 0.0, 0.0, False, False, self.dtype if not self.int4 else torch.bfloat16, None, stream)
+
     def rows(self, slots, stream=None):
         """Keys and values in `slots` (int32 [tokens]) as [tokens, kv heads, head dim]: fp32 from a 4-bit cache, else the cache's type; zeros
         for a slot outside it (-1)."""
@@ -163,36 +167,30 @@ class Cache:
         return k, v
 
 
-def _rows_ok(t, unit):
-    """Neighbouring dims, and every row on a `unit`-byte boundary."""
-    a, b, c = t.stride()
-    size = t.element_size()
-    return c == 1 and t.data_ptr() % unit == 0 and a * size % unit == 0 and b * size % unit == 0
-
-
 def _heads(q, k, v, positions, slots, cache, rope, rot, q_norm, k_norm, norm_offset, eps, interleaved, v_norm, dtype, out, stream):
-    if q.dim() != 3 or k.dim() != 3 or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2] or k.shape[1] < 1:
+    if q.dim() != 3 or k.dim() != 3:
         raise ValueError(f"q [tokens, query heads, dim] and k [tokens, KV heads, dim], got {list(q.shape)} and {list(k.shape)}")
-    T, nq, dim = q.shape
-    nkv = k.shape[1]
+    (T, nq, dim), (Tk, nkv, dim_k), source = q.shape, k.shape, q.dtype
+    if T != Tk or dim != dim_k or nkv < 1:
+        raise ValueError(f"q [tokens, query heads, dim] and k [tokens, KV heads, dim], got {list(q.shape)} and {list(k.shape)}")
     if dim not in (64, 128, 256):
         raise ValueError(f"head dim {dim} (64, 128 or 256)")
-    if q.dtype not in serve.TYPES or k.dtype != q.dtype or (v is not None and (v.dtype != q.dtype or v.shape != k.shape)):
+    if source not in serve.TYPES or k.dtype != source or (v is not None and (v.dtype != source or v.shape != k.shape)):
         raise ValueError("q, k, v: one type (fp32, bf16 or fp16), v like k")
+    (qt, qh, qd), (kt, kh, kd), (vt, vh, vd) = q.stride(), k.stride(), v.stride() if v is not None else (0, 0, 1)
+    if qd != 1 or kd != 1 or vd != 1:
+        raise ValueError("q, k, v: neighbouring dims")
     serve.whole("positions", positions, T)
     if cache is not None:
         serve.whole("slots", slots, T)
         if cache.kv_heads != nkv or cache.head_dim != dim:
             raise ValueError(f"a cache of {cache.kv_heads} heads of {cache.head_dim}, keys of {nkv} of {dim}")
     if dtype is None:
-        dtype = q.dtype if q.dtype != torch.float32 else (cache.dtype if cache is not None and not cache.int4 else torch.bfloat16)
+        dtype = source if source != torch.float32 else (cache.dtype if cache is not None and not cache.int4 else torch.bfloat16)
     if dtype != torch.bfloat16 and dtype != torch.float16:
         raise ValueError(f"dtype {dtype} (bf16 or fp16)")
-    unit = min(4, dim // 32) * q.element_size()
-    if T and not (_rows_ok(q, unit) and _rows_ok(k, unit) and (v is None or _rows_ok(v, unit))):
-        raise ValueError(f"q, k, v: neighbouring dims, rows on {unit}-byte boundaries")
     for w in (q_norm, k_norm):
-        if w is not None and (w.dtype != torch.float32 or w.shape != (dim,) or not w.is_contiguous() or w.data_ptr() % 16):
+        if w is not None and (w.dtype != torch.float32 or w.shape != (dim,) or not w.is_contiguous()):
             raise ValueError(f"q_norm, k_norm: contiguous fp32 [{dim}]")
     cos = sin = None
     angles = longest = 0
@@ -207,14 +205,14 @@ def _heads(q, k, v, positions, slots, cache, rope, rot, q_norm, k_norm, norm_off
     device = serve.on_gpu(q, k, v, positions, slots, cache.k if cache is not None else None, q_norm, k_norm, cos, sin, out)
     if out is None:
         out = serve.empty((T, nq, dim), dtype, device, stream)
-    elif out.shape != q.shape or out.dtype != dtype or not out.is_contiguous() or out.data_ptr() % 16:
+    elif out.shape != q.shape or out.dtype != dtype or not out.is_contiguous():
         raise ValueError(f"out: contiguous {dtype} {list(q.shape)}")
     k_out = serve.empty((T, nkv, dim), dtype, device, stream) if cache is None else None
     if T:
-        at = lambda t: t.data_ptr() if t is not None else 0                            # noqa: E731
-        a = serve.pack_heads(q.data_ptr(), k.data_ptr(), at(v), out.data_ptr(), at(k_out), positions.data_ptr(), at(slots), at(q_norm), at(k_norm), at(cos), at(sin),
-                             *q.stride()[:2], *k.stride()[:2], *(v.stride()[:2] if v is not None else (0, 0)), *(cache._args if cache is not None else serve.NO_CACHE), eps, norm_offset,
-                             T, nq, nkv, dim, serve.TYPES[q.dtype], serve.TYPES[dtype], rot or 0, angles, longest, bool(interleaved), bool(v_norm), device)
+        a = serve.pack_heads(q.data_ptr(), k.data_ptr(), v.data_ptr() if v is not None else 0, out.data_ptr(), k_out.data_ptr() if k_out is not None else 0, positions.data_ptr(),
+                             slots.data_ptr() if slots is not None else 0, q_norm.data_ptr() if q_norm is not None else 0, k_norm.data_ptr() if k_norm is not None else 0,
+                             cos.data_ptr() if cos is not None else 0, sin.data_ptr() if sin is not None else 0, qt, qh, kt, kh, vt, vh, *(cache._args if cache is not None else serve.NO_CACHE),
+                             eps, norm_offset, T, nq, nkv, dim, serve.TYPES[source], serve.TYPES[dtype], rot or 0, angles, longest, bool(interleaved), bool(v_norm), device)
         code = serve.lib().mk_heads(a, serve.raw_stream(device, stream))
         if code:
             _lib.check(code)
@@ -299,13 +297,14 @@ def attend(q, cache, table, context, starts=None, max_new=None, scale=None, wind
     lib = serve.lib()
     if out is None:
         out = serve.empty(q.shape, q.dtype, device, stream)
-    elif out.shape != q.shape or out.dtype != q.dtype or (T and not _rows_ok(out, 16)):
-        raise ValueError(f"out: {q.dtype} {list(q.shape)}, neighbouring dims, rows on 16-byte boundaries")
+    elif out.shape != q.shape or out.dtype != q.dtype:
+        raise ValueError(f"out: {q.dtype} {list(q.shape)}")
     if T == 0:
         return out
-    if not _rows_ok(q, 16):
-        raise ValueError("q: neighbouring dims, rows on 16-byte boundaries")
-    fixed = (*q.stride()[:2], *out.stride()[:2], table.stride(0), *cache._args, 0, dim ** -0.5 if scale is None else scale, serve.TYPES[q.dtype], R, T, nq, pages, min(max_new, T),
+    (qt, qh, qd), (ot, oh, od) = q.stride(), out.stride()
+    if qd != 1 or od != 1:
+        raise ValueError("q, out: neighbouring dims")
+    fixed = (qt, qh, ot, oh, table.stride(0), *cache._args, 0, dim ** -0.5 if scale is None else scale, serve.TYPES[q.dtype], R, T, nq, pages, min(max_new, T),
              min(window, 2 ** 31 - 1), min(sinks, 2 ** 31 - 1), device)
     front = (q.data_ptr(), out.data_ptr(), table.data_ptr(), context.data_ptr(), starts.data_ptr() if starts is not None else 0)
     need = _bytes.get((device, dim))                               # it depends on nothing else

@@ -20,6 +20,7 @@ import math
 import torch
 
 from ..stage import desc as D
+from ..stage.kv import FourBitLayers, SequenceCalls, SharedPages
 from ..stage.runtime import PeerMailbox, Program, Runtime
 from .dims import DK, DV, HD, ROT, Dims
 from .pack import Packed
@@ -42,18 +43,25 @@ def attn_chunk(maxlen, tasks_per_pos, grid):
     return max(16, min(D.query("ATTN_MAX_CHUNK"), cp))
 
 
-class Engine:
+class Engine(SequenceCalls):
     def __init__(self, PK: Packed, M: int, maxlen: int = 4096, layers=None, device="cuda", block: int = KV_BLOCK,
-                 group=None, lm_head: bool = True, spin_limit_ms=2000, mailbox=None, kv_layout="pages", kv_block=KV_BLOCK):
+                 group=None, lm_head: bool = True, spin_limit_ms=2000, mailbox=None, kv_layout="pages", kv_block=KV_BLOCK,
+                 kv_dtype="bf16", kv_pages=None):
         """`kv_layout="serving"` keeps the KV cache as [page][position][kv head][head dim] with `kv_block` positions per
         page (a power of two), the layout a serving stack's paged attention uses; the default is this kernel's own
-        [page][kv head][64][head dim]."""
+        [page][kv head][64][head dim].
+
+        `kv_pages=N` keeps N pages (page 0 among them) that the sequences share as they grow, instead of M times the pages of `maxlen`; a sequence
+        for which there is none waits (its position stays, its logits of that step are undefined).  `kv_dtype="int4"` keeps keys and values in 4 bits
+        (`paged.Cache`); its attention layers run outside the stage kernel."""
         if block != KV_BLOCK:
             raise ValueError(f"KV pages hold {KV_BLOCK} positions (kv_block sets the page size of the serving layout)")
         if kv_layout not in ("pages", "serving") or kv_block < 8 or kv_block & (kv_block - 1):
             raise ValueError("kv_layout: 'pages' or 'serving'; kv_block: a power of two >= 8")
         if kv_layout == "pages":
             kv_block = KV_BLOCK
+        if kv_dtype not in ("bf16", "int4") or (kv_dtype == "int4" and (kv_layout != "pages" or PK.tp > 1)):
+            raise ValueError("kv_dtype: 'bf16', or 'int4' with the 'pages' layout on one GPU")
         self.kv_layout, self.kv_block = kv_layout, kv_block
         if not 1 <= M <= D.MAX_BATCH:
             raise ValueError(f"M must lie in [1, {D.MAX_BATCH}]")
@@ -86,13 +94,20 @@ class Engine:
         cos, sin = rope_tables(s.theta, self.maxlen, dev)
         pr.hold(cos), pr.hold(sin)
         g = torch.Generator().manual_seed(0)
-        self.bt = (torch.randperm(M * nb, generator=g) + 1).reshape(M, nb).to(torch.int32).to(dev)
+        int4, pages = kv_dtype == "int4", M * nb + 1 if kv_pages is None else kv_pages
+        if int4 or kv_pages is not None:
+            self.pages = SharedPages(M, pages, nb, KB, dev)
+            self.bt = self.pages.pool.table
+        else:
+            self.bt = (torch.randperm(M * nb, generator=g) + 1).reshape(M, nb).to(torch.int32).to(dev)
         pr.hold(self.bt)
         n_att = sum(s.is_attn(i) for i in range(self.layers))
         n_gdn = self.layers - n_att
-        kv_shape = (M * nb + 1, d.nkv, KB, HD) if kv_layout == "pages" else (M * nb + 1, KB, d.nkv, HD)
-        self.k_cache = z(n_att, *kv_shape, dtype=torch.bfloat16)
-        self.v_cache = z(n_att, *kv_shape, dtype=torch.bfloat16)
+        kv_shape = (pages, d.nkv, KB, HD) if kv_layout == "pages" else (pages, KB, d.nkv, HD)
+        if not int4:
+            self.k_cache = z(n_att, *kv_shape, dtype=torch.bfloat16)
+            self.v_cache = z(n_att, *kv_shape, dtype=torch.bfloat16)
+        four_bit = []
         kv_fields = {} if kv_layout == "pages" else dict(KV_BLOCK=KB, KV_S_PAGE=KB * d.nkv * HD, KV_S_HEAD=HD, KV_S_POS=d.nkv * HD)
         self.conv = z(n_gdn, M, d.conv_dim, 4)
         self.ssm = z(n_gdn, M, d.nvh, DV, DK)
@@ -118,9 +133,10 @@ class Engine:
                                      Q_BF16=1, MAX_CHUNKS=max_chunks, **kv_fields),
                               f=dict(EPS=s.eps, SCALE=HD ** -0.5),
                               p=dict(A_Y=self.y.data_ptr(), A_Y2=self.y2.data_ptr(), Q_NORM=sm("self_attn.q_norm.weight").data_ptr(),
-                                     K_NORM=sm("self_attn.k_norm.weight").data_ptr(), K_CACHE=self.k_cache[ai].data_ptr(),
-                                     V_CACHE=self.v_cache[ai].data_ptr(), BLOCK_TABLE=self.bt.data_ptr(), ROPE_COS=cos.data_ptr(),
+                                     K_NORM=sm("self_attn.k_norm.weight").data_ptr(), K_CACHE=0 if int4 else self.k_cache[ai].data_ptr(),
+                                     V_CACHE=0 if int4 else self.v_cache[ai].data_ptr(), BLOCK_TABLE=self.bt.data_ptr(), ROPE_COS=cos.data_ptr(),
                                      ROPE_SIN=sin.data_ptr(), A_PART=a_part.data_ptr(), A_CNT=a_cnt.data_ptr())))
+                four_bit.append(dict(index=len(pr.stages) - 1, q_norm=sm("self_attn.q_norm.weight"), k_norm=sm("self_attn.k_norm.weight")))
                 w, meta = PK.mats[(i, "o")]
                 pr.gemv("o", w, meta, self.y2, self.h, x_stride=y2w, out_stride=H, epilogue=D.MKS_E_RESID, out_ssq=self.ssq,
                         n_valid=H, allreduce=ar)
@@ -157,18 +173,22 @@ class Engine:
         self.peer = mailbox if mailbox is not None else (PeerMailbox(group, rank, tp, dev) if tp > 1 else None)
         self.rt = Runtime(pr, mailbox=self.peer, tp=tp, rank=rank, spin_limit_ms=spin_limit_ms)
         self.pos = self.rt.pos
+        if int4 and four_bit:
+            self.kv4 = FourBitLayers(self, four_bit, (cos, sin), pages, KB, nb)
 
     # ------------------------------------------------------------------------------------------------
     def reset(self):
         for t in (self.conv, self.ssm):
             t.zero_()
         self.rt.reset()
+        if self.pages is not None:
+            self.pages.reset()
 
     def step(self, tok: torch.Tensor, valid=None, stream=None):
         """One decode step for all M rows.  tok: [M] int.  Returns fp32 logits [M, vocab of this rank] (a view,
         overwritten by the next step)."""
         self.rt.tok[: self.M].copy_(tok.to(device=self.device, dtype=torch.int32))
-        self.rt.launch(1, stream=stream, row_valid=self._rows(valid))
+        self._advance(self._rows(valid), stream)
         return self.logits
 
     def _rows(self, valid):
@@ -181,14 +201,19 @@ class Engine:
         self.rowv[: self.M].copy_(torch.as_tensor(valid).to(device=self.device, dtype=torch.int32))
         return self.rowv
 
-    def generate(self, tok: torch.Tensor, n_steps: int):
+    def generate(self, tok: torch.Tensor, n_steps: int, temperature=0.0, top_k=0, top_p=1.0, min_p=0.0, seed=0):
         """`n_steps` decode steps in one launch: step 0 feeds `tok`, every later step the greedy choice of the
-        step before.  Returns the chosen ids [n_steps, M] (int32, on the device)."""
+        step before.  Returns the chosen ids [n_steps, M] (int32, on the device).  With a temperature the tokens are sampled (`sampling.sample`:
+        top_k, top_p, min_p; uniform numbers from `seed`), a launch or two per step."""
         if not self.lm_head:
             raise RuntimeError("generate needs the LM head")
+        if temperature > 0:
+            if self.PK.tp > 1:
+                raise RuntimeError("sampling needs all logits on one GPU")
+            return self._advance_sampled(tok, n_steps, temperature, top_k, top_p, min_p, seed)
         out = torch.zeros(n_steps, self.M, dtype=torch.int32, device=self.device)
         self.rt.tok[: self.M].copy_(tok.to(device=self.device, dtype=torch.int32))
-        self.rt.launch(n_steps, tokens_out=out)
+        self._advance_greedy(n_steps, out)
         return out
 
     def prefill(self, prompts):
@@ -198,7 +223,7 @@ class Engine:
         if len(prompts) != self.M or len({len(p) for p in prompts}) != 1 or not prompts[0]:
             raise ValueError(f"prefill takes {self.M} prompts of one common, non-zero length")
         toks = torch.tensor(prompts, dtype=torch.int32).t().contiguous().to(self.device)      # [L, M]
-        self.rt.prefill(toks)
+        self._take_in(toks)
         self._prompt = toks                                  # alive until the launch has run
         return self.logits
 
@@ -224,6 +249,8 @@ class Engine:
         """K, V of attention layer ai for positions [0, n) of sequence m: [kv heads, n, 256] fp32."""
         pos = torch.arange(n, device=self.device)
         blk, off = self.bt[m].long()[pos // self.kv_block], pos % self.kv_block
+        if self.kv4 is not None:
+            return tuple(t.transpose(0, 1) for t in self.kv4.caches[ai].rows((blk * self.kv_block + off).int()))
         if self.kv_layout == "pages":
             return self.k_cache[ai][blk, :, off].transpose(0, 1).float(), self.v_cache[ai][blk, :, off].transpose(0, 1).float()
         return self.k_cache[ai][blk, off].transpose(0, 1).float(), self.v_cache[ai][blk, off].transpose(0, 1).float()
@@ -234,5 +261,6 @@ class Engine:
         body, head = self.PK.weight_bytes()
         d = self.d
         state = 2 * 4 * self.ssm.shape[0] * d.nvh * DV * DK
-        kv = self.k_cache.shape[0] * 2 * d.nkv * HD * 2 * context
+        per_value = 2 if self.kv4 is None else 4.5 / 8                   # 4 bits and a share of the scales
+        kv = int(sum(self.shape.is_attn(i) for i in range(self.layers)) * 2 * d.nkv * HD * per_value * context)
         return body + head + self.M * (state + kv)

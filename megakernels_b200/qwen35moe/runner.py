@@ -19,24 +19,25 @@ group order, into the residual stream.
 import torch
 
 from ..stage import desc as D
+from ..stage.kv import FourBitLayers, SequenceCalls, SharedPages
 from ..stage.runtime import Program, Runtime
 from ..qwen27b.runner import KV_BLOCK, attn_chunk, rope_tables
 from .dims import DK, DV, HD, ROT
 from .pack import Packed
 
 
-class Engine:
+class Engine(SequenceCalls):
     def __init__(self, PK: Packed, M: int, maxlen: int = 4096, layers=None, device="cuda", lm_head: bool = True,
-                 spin_limit_ms=2000, exact_inputs=False, kv_dtype="bf16"):
+                 spin_limit_ms=2000, exact_inputs=False, kv_dtype="bf16", kv_pages=None):
         """`exact_inputs=True` feeds the FP8 GEMVs fp32-exact inputs as two fp16 pieces (M <= 4) and keeps the conv
         history unrounded: the arithmetic of the reference's exact mode.  The default rounds GEMV inputs and the
-        conv history to bf16, the model's own dtype."""
+        conv history to bf16, the model's own dtype.  `kv_pages` and `kv_dtype="int4"`: see `qwen27b.Engine`."""
         if not 1 <= M <= D.MAX_BATCH:
             raise ValueError(f"M must lie in [1, {D.MAX_BATCH}]")
         if exact_inputs and M > 4:
             raise ValueError("two-piece inputs occupy two MMA columns per sequence: M <= 4")
-        if kv_dtype not in ("bf16", "fp32"):
-            raise ValueError("kv_dtype: 'bf16' or 'fp32'")
+        if kv_dtype not in ("bf16", "fp32", "int4") or (kv_dtype == "int4" and exact_inputs):
+            raise ValueError("kv_dtype: 'bf16', 'fp32', or 'int4' without exact_inputs")
         if not torch.cuda.is_available():
             raise RuntimeError("the megakernel needs a CUDA device; there is no CPU path")
         self.PK, self.M = PK, M
@@ -67,13 +68,20 @@ class Engine:
         cos, sin = rope_tables(s.theta, self.maxlen, dev)
         pr.hold(cos), pr.hold(sin)
         g = torch.Generator().manual_seed(0)
-        self.bt = (torch.randperm(M * nb, generator=g) + 1).reshape(M, nb).to(torch.int32).to(dev)
+        int4, pages = kv_dtype == "int4", M * nb + 1 if kv_pages is None else kv_pages
+        if int4 or kv_pages is not None:
+            self.pages = SharedPages(M, pages, nb, KV_BLOCK, dev)
+            self.bt = self.pages.pool.table
+        else:
+            self.bt = (torch.randperm(M * nb, generator=g) + 1).reshape(M, nb).to(torch.int32).to(dev)
         pr.hold(self.bt)
         n_att = sum(s.is_attn(i) for i in range(self.layers))
         n_gdn = self.layers - n_att
         kvt = torch.bfloat16 if kv_dtype == "bf16" else torch.float32
-        self.k_cache = z(n_att, M * nb + 1, s.nkv, KV_BLOCK, HD, dtype=kvt)
-        self.v_cache = z(n_att, M * nb + 1, s.nkv, KV_BLOCK, HD, dtype=kvt)
+        if not int4:
+            self.k_cache = z(n_att, pages, s.nkv, KV_BLOCK, HD, dtype=kvt)
+            self.v_cache = z(n_att, pages, s.nkv, KV_BLOCK, HD, dtype=kvt)
+        four_bit = []
         self.conv = z(n_gdn, M, s.conv_dim, 4)
         self.ssm = z(n_gdn, M, s.nvh, DV, DK)
         qpk = s.nq // s.nkv
@@ -99,9 +107,10 @@ class Engine:
                                      ROPE_PAIRS=ROT // 2, Q_BF16=int(not exact_inputs), MAX_CHUNKS=max_chunks),
                               f=dict(EPS=s.eps, SCALE=HD ** -0.5),
                               p=dict(A_Y=self.y.data_ptr(), A_Y2=self.y2.data_ptr(), Q_NORM=sm("self_attn.q_norm.weight").data_ptr(),
-                                     K_NORM=sm("self_attn.k_norm.weight").data_ptr(), K_CACHE=self.k_cache[ai].data_ptr(),
-                                     V_CACHE=self.v_cache[ai].data_ptr(), BLOCK_TABLE=self.bt.data_ptr(), ROPE_COS=cos.data_ptr(),
+                                     K_NORM=sm("self_attn.k_norm.weight").data_ptr(), K_CACHE=0 if int4 else self.k_cache[ai].data_ptr(),
+                                     V_CACHE=0 if int4 else self.v_cache[ai].data_ptr(), BLOCK_TABLE=self.bt.data_ptr(), ROPE_COS=cos.data_ptr(),
                                      ROPE_SIN=sin.data_ptr(), A_PART=a_part.data_ptr(), A_CNT=a_cnt.data_ptr())))
+                four_bit.append(dict(index=len(pr.stages) - 1, q_norm=sm("self_attn.q_norm.weight"), k_norm=sm("self_attn.k_norm.weight")))
                 w, meta = PK.mats[(i, "o")]
                 pr.gemv("o", w, meta, self.y2, self.h, x_stride=y2w, out_stride=H, epilogue=D.MKS_E_RESID, out_ssq=self.ssq,
                         n_valid=H, pieces=pc(meta))
@@ -148,18 +157,22 @@ class Engine:
         self.lm_head = lm_head
         self.rt = Runtime(pr, spin_limit_ms=spin_limit_ms)
         self.pos = self.rt.pos
+        if int4 and four_bit:
+            self.kv4 = FourBitLayers(self, four_bit, (cos, sin), pages, KV_BLOCK, nb)
 
     # ------------------------------------------------------------------------------------------------
     def reset(self):
         for t in (self.conv, self.ssm):
             t.zero_()
         self.rt.reset()
+        if self.pages is not None:
+            self.pages.reset()
 
     def step(self, tok: torch.Tensor, valid=None, stream=None):
         """One decode step for all M rows.  tok: [M] int.  Returns fp32 logits [M, vocab] (a view, overwritten by
         the next step)."""
         self.rt.tok[: self.M].copy_(tok.to(device=self.device, dtype=torch.int32))
-        self.rt.launch(1, stream=stream, row_valid=self._rows(valid))
+        self._advance(self._rows(valid), stream)
         return self.logits
 
     def _rows(self, valid):
@@ -172,14 +185,16 @@ class Engine:
         self.rowv[: self.M].copy_(torch.as_tensor(valid).to(device=self.device, dtype=torch.int32))
         return self.rowv
 
-    def generate(self, tok: torch.Tensor, n_steps: int):
-        """`n_steps` decode steps in one launch, every later step fed the greedy choice of the one before.
-        Returns the chosen ids [n_steps, M] (int32, on the device)."""
+    def generate(self, tok: torch.Tensor, n_steps: int, temperature=0.0, top_k=0, top_p=1.0, min_p=0.0, seed=0):
+        """`n_steps` decode steps in one launch, every later step fed the greedy choice of the one before
+        (with a temperature: tokens sampled as `qwen27b.Engine.generate` does).  Returns the chosen ids [n_steps, M] (int32, on the device)."""
         if not self.lm_head:
             raise RuntimeError("generate needs the LM head")
+        if temperature > 0:
+            return self._advance_sampled(tok, n_steps, temperature, top_k, top_p, min_p, seed)
         out = torch.zeros(n_steps, self.M, dtype=torch.int32, device=self.device)
         self.rt.tok[: self.M].copy_(tok.to(device=self.device, dtype=torch.int32))
-        self.rt.launch(n_steps, tokens_out=out)
+        self._advance_greedy(n_steps, out)
         return out
 
     def prefill(self, prompts):
@@ -187,7 +202,7 @@ class Engine:
         if len(prompts) != self.M or len({len(p) for p in prompts}) != 1 or not prompts[0]:
             raise ValueError(f"prefill takes {self.M} prompts of one common, non-zero length")
         toks = torch.tensor(prompts, dtype=torch.int32).t().contiguous().to(self.device)
-        self.rt.prefill(toks)
+        self._take_in(toks)
         self._prompt = toks
         return self.logits
 
@@ -209,6 +224,8 @@ class Engine:
     def kv_rows(self, ai, m, n):
         pos = torch.arange(n, device=self.device)
         blk, off = self.bt[m].long()[pos // KV_BLOCK], pos % KV_BLOCK
+        if self.kv4 is not None:
+            return tuple(t.transpose(0, 1) for t in self.kv4.caches[ai].rows((blk * KV_BLOCK + off).int()))
         return self.k_cache[ai][blk, :, off].transpose(0, 1).float(), self.v_cache[ai][blk, :, off].transpose(0, 1).float()
 
     def bytes_per_step(self, context, distinct_experts=None):
@@ -220,5 +237,6 @@ class Engine:
         n = distinct_experts if distinct_experts is not None else min(s.experts, self.M * s.topk)
         routed = sum(m["stride"] * n for (k, (_, m)) in self.PK.mats.items() if k[1].startswith("ex_"))
         state = 2 * 4 * self.ssm.shape[0] * s.nvh * DV * DK
-        kv = self.k_cache.shape[0] * 2 * s.nkv * HD * self.k_cache.element_size() * context
+        per_value = self.k_cache.element_size() if self.kv4 is None else 4.5 / 8     # 4 bits and a share of the scales
+        kv = int(sum(s.is_attn(i) for i in range(self.layers)) * 2 * s.nkv * HD * per_value * context)
         return dense + routed + head + self.M * (state + kv)

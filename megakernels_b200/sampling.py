@@ -73,3 +73,17 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, stream=Non
         if code:
             _lib.check(code)
     return Sample(ids, logprobs, kept)
+
+
+def continue_from(step, tok, n_steps, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, seed=0):
+    """`n_steps` sampled tokens of every sequence: `step(tok [rows]) -> logits [rows, vocab]` takes one token of each in.  The uniform numbers
+    are those of a generator seeded with `seed`.  Returns int32 [n_steps, rows] on the device; nothing waits for it."""
+    check_settings(temperature, top_k, top_p, min_p)
+    rows, device = tok.shape[0], tok.device
+    u = torch.rand(n_steps, rows, generator=torch.Generator(device=device).manual_seed(seed), device=device)
+    settings = [torch.full((rows,), v, dtype=torch.int32 if n == "top_k" else torch.float32, device=device) for n, v in zip(_NEUTRAL, (temperature, top_k, top_p, min_p))]
+    out = torch.empty(n_steps, rows, dtype=torch.int32, device=device)
+    for t in range(n_steps):
+        out[t] = sample(step(tok), u[t], *settings).ids
+        tok = out[t].clamp(min=0)                                  # (a padding row's logits are nothing in particular)
+    return out

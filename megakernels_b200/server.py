@@ -5,7 +5,7 @@
 
 Endpoints and request fields of the reference's server (`qwen3.5-0.8b/qwen_mk/server.py:27-209`): GET /v1/models and
 /health; POST /v1/chat/completions with `messages`, `stream`, `max_tokens` / `max_completion_tokens`, `temperature`,
-`seed`, `tools`, `enable_thinking` (also under `chat_template_kwargs`).  Replies carry `reasoning_content` for a
+`seed`, `top_p`, `top_k`, `min_p`, `tools`, `enable_thinking` (also under `chat_template_kwargs`).  Replies carry `reasoning_content` for a
 `<think>` block and `tool_calls` parsed from the model's XML tool-call format.  One engine, one sequence: requests
 are served one at a time (the session's lock), and consecutive requests of a conversation reuse the state.
 """
@@ -19,6 +19,7 @@ import uuid
 from http.server import BaseHTTPRequestHandler, ThreadingHTTPServer
 
 from .chat import TextStream
+from .sampling import check_settings
 
 MODEL_ID = "qwen3.5-0.8b-megakernel-b200"
 _CALL = re.compile(r"<tool_call>\s*<function=([^>\s]+)>(.*?)</function>\s*</tool_call>", re.S)
@@ -80,6 +81,20 @@ def settled(text, tag):
     return text
 
 
+def filters_of(req):
+    """What a request asks of the choice of tokens beyond a temperature; ValueError if it means nothing."""
+    found = {}
+    for name, kind, neutral in (("top_k", int, 0), ("top_p", float, 1.0), ("min_p", float, 0.0)):
+        if req.get(name) is not None:
+            value = kind(req[name])
+            if value != neutral:
+                found[name] = value
+    if found.get("top_k") == -1:                # what some clients send for "all"
+        del found["top_k"]
+    check_settings(**found)
+    return found
+
+
 def complete(session, req):
     """The non-streaming reply object for a parsed request body."""
     messages = plain_messages(req["messages"])
@@ -87,7 +102,7 @@ def complete(session, req):
     tools = req.get("tools") or None
     prompt = session.encode(session.render(messages, enable_thinking=think, tools=tools))
     budget = int(req.get("max_completion_tokens") or req.get("max_tokens") or 2048)
-    ids = list(session.stream(prompt, max_new_tokens=budget, temperature=float(req.get("temperature", 0.7)), seed=req.get("seed")))
+    ids = list(session.stream(prompt, max_new_tokens=budget, temperature=float(req.get("temperature", 0.7)), seed=req.get("seed"), **filters_of(req)))
     finish = "stop" if ids and ids[-1] in session.stop_ids else "length"
     text, reasoning = split_thinking(session.tok.decode([t for t in ids if t not in session.stop_ids]))
     content, calls = extract_tool_calls(text)
@@ -119,7 +134,7 @@ def stream_chunks(session, req):
     sent_thought = sent_answer = 0
     answer_from = None if think else 0          # index in `text` where the visible answer begins
     finish = "length"
-    for t in session.stream(prompt, max_new_tokens=budget, temperature=float(req.get("temperature", 0.7)), seed=req.get("seed")):
+    for t in session.stream(prompt, max_new_tokens=budget, temperature=float(req.get("temperature", 0.7)), seed=req.get("seed"), **filters_of(req)):
         if t in session.stop_ids:               # always the last id; keep iterating so the session closes its ledger
             finish = "stop"
             continue
@@ -185,7 +200,8 @@ class Handler(BaseHTTPRequestHandler):
             req = json.loads(self.rfile.read(int(self.headers.get("Content-Length", 0))) or b"{}")
             if not isinstance(req.get("messages"), list):
                 raise KeyError("messages")
-        except (ValueError, KeyError) as e:
+            filters_of(req)
+        except (ValueError, TypeError, KeyError) as e:
             return self._reply(400, {"error": {"message": f"bad request: {e}"}})
         if not req.get("stream"):
             return self._reply(200, complete(self.session, req))

@@ -124,8 +124,8 @@ class ChatSession:
         return len(want) - start
 
     # ---- generation
-    def stream(self, prompt_ids, max_new_tokens=512, temperature=0.7, seed=None, chunk=16):
-        """Generated ids for a tokenised prompt, one by one.  Run it to the end: only then does the session know
+    def stream(self, prompt_ids, max_new_tokens=512, temperature=0.7, seed=None, chunk=16, **filters):
+        """Generated ids for a tokenised prompt, one by one (`filters`: top_k, top_p, min_p as `Megakernel.generate` takes them).  Run it to the end: only then does the session know
         what the engine has absorbed (an abandoned generator leaves the ledger unknown and the next request goes
         back to a snapshot)."""
         seed = (time.time_ns() & 0x7FFFFFFF) if seed is None else seed
@@ -137,7 +137,7 @@ class ChatSession:
             produced = []
             self.fed = None
             for t in self.mk.generate([prompt_ids[-1]], max_new_tokens=max_new_tokens, temperature=temperature, seed=seed,
-                                      stop_ids=self.stop_ids, chunk=chunk, spec=self.spec):
+                                      stop_ids=self.stop_ids, chunk=chunk, spec=self.spec, **filters):
                 produced.append(t)
                 yield t
             # all but the last produced id have been fed (the last is a stop id, or the id chosen when the budget ran out)

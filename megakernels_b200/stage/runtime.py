@@ -183,14 +183,14 @@ class Runtime:
             if t.dtype == torch.int32:
                 t.zero_()
 
-    def launch(self, n_steps=1, tokens_out=None, prof=None, stream=None, n_stages=None, prof_cta=0, tokens_in=None, row_valid=None, program=None):
-        """`n_stages` runs only a prefix of the program (one step; for stage-by-stage checks in tests); `program`, a (device
-        copy, records) pair whose records all end in a barrier, another one."""
+    def launch(self, n_steps=1, tokens_out=None, prof=None, stream=None, n_stages=None, prof_cta=0, tokens_in=None, row_valid=None, program=None, pos=None):
+        """`n_stages` runs only a prefix of the program (one step; for stage-by-stage checks in tests); `program`, what
+        `upload` returned, another one; `pos`, other positions than the runtime's."""
         full = n_stages is None and program is None
         n_stages = program[1] if program is not None else (self.n_stages if full else n_stages)
         assert full or n_steps == 1
         a = D.StageArgs(program=(program[0] if program is not None else self.program_dev).data_ptr(), n_stages=n_stages, batch=self.M, n_steps=n_steps,
-                        device=self.device.index, tok=self.tok.data_ptr(), pos=self.pos.data_ptr(),
+                        device=self.device.index, tok=self.tok.data_ptr(), pos=(pos if pos is not None else self.pos).data_ptr(),
                         tokens_out=tokens_out.data_ptr() if tokens_out is not None else 0, barrier=self.bar.data_ptr(),
                         barrier_base=self.bar_base, status=self.status.data_ptr(), spin_limit_ns=self.spin_limit_ns,
                         prof=prof.data_ptr() if prof is not None else 0, tp=self.tp, rank=self.rank, ar_base=self.ar_base,
@@ -205,7 +205,7 @@ class Runtime:
         _lib.check(self.lib.mk_stage_launch(ctypes.byref(a), ctypes.c_void_p(st.cuda_stream)))
         nb, na = self.barriers_per_step, self.allreduces_per_step
         if program is not None:
-            nb, na = n_stages, 0
+            nb, na = program[2], 0
         elif not full:
             nb = sum(1 for d in self.prog.stages[:n_stages] if not d.flags & D.MKS_FLAG_NO_BARRIER)
             na = sum(1 for d in self.prog.stages[:n_stages] if d.op == D.MKS_OP_GEMV and d.i[D.MKS_I_ALLREDUCE])
@@ -226,12 +226,8 @@ class Runtime:
             need = int(self.lib.mk_stage_prefill_bytes(self.host, self.n_stages, self.M, each, self.device.index))
             if need < 0 and need != _lib.MK_ERR_UNSUPPORTED:
                 _lib.check(need)
-        if need > 0 and (self._workspace is None or self._workspace.numel() < need):
-            self._workspace = None
-            try:
-                self._workspace = torch.empty(need, dtype=torch.uint8, device=self.device)
-            except torch.cuda.OutOfMemoryError:
-                need = -1                       # no memory left for it: steps need none
+        if need > 0 and not self.workspace_room(need):
+            need = -1                           # steps need none
         self.tok[: self.M].copy_(tokens[0])
         if need < 0:
             return self.launch(L, tokens_in=tokens)
@@ -252,9 +248,24 @@ class Runtime:
             first, last = D.StageDesc.from_buffer_copy(self.host[0]), self.host[self.n_stages - 1]
             first.i[D.K["MKS_I_HIDDEN"]] = 0
             records = [first] + ([last] if last.op == D.MKS_OP_GEMV and last.i[D.MKS_I_EPILOGUE] == D.MKS_E_LOGITS else [])
-            arr = (D.StageDesc * len(records))(*records)
-            self._head = torch.frombuffer(bytearray(bytes(arr)), dtype=torch.uint8).to(self.device), len(records)
+            self._head = self.upload(records)
         return self._head
+
+    def upload(self, records):
+        """(device copy, number of records, barriers of a step) of a program other than the runtime's own, for `launch`; without all-reduces."""
+        arr = (D.StageDesc * len(records))(*records)
+        barriers = sum(1 for d in records if not d.flags & D.MKS_FLAG_NO_BARRIER)
+        return torch.frombuffer(bytearray(bytes(arr)), dtype=torch.uint8).to(self.device), len(records), barriers
+
+    def workspace_room(self, need):
+        """Makes the workspace of the token-parallel path `need` bytes large; False where the device has no memory left for it."""
+        if self._workspace is None or self._workspace.numel() < need:
+            self._workspace = None
+            try:
+                self._workspace = torch.empty(need, dtype=torch.uint8, device=self.device)
+            except torch.cuda.OutOfMemoryError:
+                return False
+        return True
 
     def check(self):
         """Synchronise and raise if a device-side wait ran out in any launch so far."""
