@@ -646,6 +646,6 @@ extern "C" int mk_attend(const mk_attend_args* a, void* stream) {
     A.spin_limit_ns = a->spin_limit_ns > 0 ? a->spin_limit_ns : 2000000000ll;
     A.scale_log2 = a->scale * 1.4426950408889634f;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if ((int64_t)a->max_new * A.per > 32) return launch_rows(A, c.type, c.head_dim, st);
+    if ((int64_t)a->max_new * A.per > 32) return launch_rows(A, c.type, c.head_dim, sms, st);
     return c.head_dim == 64 ? launch_kind<64>(A, c.type, sms, st) : (c.head_dim == 128 ? launch_kind<128>(A, c.type, sms, st) : launch_kind<256>(A, c.type, sms, st));
 }

@@ -82,6 +82,6 @@ template <int I> __device__ __forceinline__ uint32_t codes(uint32_t w) {
 enum { K_BF16, K_F16, K_INT4 };
 
 // mk_attend_rows.cu
-int launch_rows(const AttendArgs& A, int type, int head_dim, cudaStream_t st);
+int launch_rows(const AttendArgs& A, int type, int head_dim, int sms, cudaStream_t st);
 
 }  // namespace mkv

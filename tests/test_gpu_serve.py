@@ -290,6 +290,24 @@ def test_attend_what_nobody_sees_is_not_looked_at(kind):
     assert bool((got[3] == 0).all()) and bool((got[4:9] == 0).all())
 
 
+@pytest.mark.parametrize("kind,dtype,layout", [("bf16", torch.bfloat16, "pages"), ("fp16", torch.float16, "serving"), ("int4", torch.bfloat16, "pages")])
+@pytest.mark.parametrize("nq,nkv,dim,page", [(24, 4, 256, 64), (8, 8, 128, 16), (32, 4, 64, 256)])
+def test_attend_more_blocks_than_the_gpu_takes_at_once(kind, dtype, layout, nq, nkv, dim, page):
+    """Every block of rows goes on where another one has been: requests of no, one and many queries, some of them with fewer positions than queries or none at all."""
+    rng = torch.Generator().manual_seed(dim)
+    counts = [int(x) for x in torch.randint(0, 130, (90,), generator=rng)] + [300, 0, 1, 2, 700]
+    contexts = [c + int(x) for c, x in zip(counts, torch.randint(0, 500, (95,), generator=rng))]
+    for r in (3, 4, 5, 6, 7, 40):
+        contexts[r] = 0
+    contexts[20], contexts[21] = counts[20] // 2, max(counts[21] - 1, 0)
+    for window, sinks in ((0, 0), (100, 5)):
+        cache, k, v, table, context, starts, q = case(kind, dtype, nq, nkv, dim, page, contexts, counts, window, sinks, seed=window, layout=layout)
+        got = paged.attend(q, cache, table, context, starts=starts, window=window, sinks=sinks)
+        paged.check()
+        compare(got, R.attend(q, k, v, table, context, starts, dim ** -0.5, window, sinks), cache, v, dtype, many=True)
+        assert torch.equal(got, paged.attend(q, cache, table, context, starts=starts, window=window, sinks=sinks))
+
+
 def test_attend_leaves_other_rows_alone_and_takes_strides():
     cache, k, v, table, context, starts, q = case("bf16", torch.bfloat16, 4, 2, 64, 16, [50, 20], [2, 3], 0, 0, seed=3, layout="serving")
     wide = torch.full((8, 4, 192), 7.0, dtype=torch.bfloat16, device=DEV)
