@@ -87,7 +87,8 @@ int mk_cache_rows(const mk_cache* cache, uint64_t slots, int tokens, uint64_t k_
  * and sees the cached keys j <= position with j > position - window or j < sinks (window 0: all of them).
  * out = sum_j softmax_j(scale q k_j) v_j, query head h with KV head h / (q_heads / kv_heads); a query that sees nothing gives
  * zeros.  Keys in a page that the table does not place inside the cache are not seen.  Rows of out outside
- * [starts[0], starts[requests]) are left alone. */
+ * [starts[0], starts[requests]) are left alone.  What no query of the call sees is not looked at and may hold anything; values
+ * that some query sees have to be finite (queries of a tile that do not see them multiply them by 0).  scale > 0. */
 typedef struct {
     uint64_t q, out;                 /* [tokens][q_heads][head_dim] of `type`                                  */
     uint64_t table, context, starts; /* i32[requests][table_stride], i32[requests], i32[requests + 1] or 0     */

@@ -620,6 +620,8 @@ extern "C" int mk_attend(const mk_attend_args* a, void* stream) {
     const int64_t strides[] = {a->q_tok, a->q_head, a->out_tok, a->out_head};
     for (int64_t s : strides)
         if (s < 0 || s % 8) return vfail(MK_ERR_BADARG, "mk_attend: stride %lld (a multiple of 8 elements)", (long long)s);
+    if ((a->tokens > 1 && a->out_tok < a->cache.head_dim) || (a->q_heads > 1 && a->out_head < a->cache.head_dim))
+        return vfail(MK_ERR_BADARG, "mk_attend: rows of out overlap at strides %lld, %lld", (long long)a->out_tok, (long long)a->out_head);
     if (a->table_stride < a->max_pages && a->requests > 1) return vfail(MK_ERR_BADARG, "mk_attend: table rows %lld apart hold no %d pages", (long long)a->table_stride, a->max_pages);
     if (a->tokens == 0) return MK_OK;
     MKV_DEVICE(a->device);

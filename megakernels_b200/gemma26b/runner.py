@@ -193,7 +193,7 @@ class Engine(SequenceCalls):
     def generate(self, tok: torch.Tensor, n_steps: int, temperature=0.0, top_k=0, top_p=1.0, min_p=0.0, seed=0):
         if not self.lm_head:
             raise RuntimeError("generate needs the LM head")
-        if temperature > 0:
+        if self._sampled(temperature, top_k, top_p, min_p):
             return self._advance_sampled(tok, n_steps, temperature, top_k, top_p, min_p, seed)
         out = torch.zeros(n_steps, self.M, dtype=torch.int32, device=self.device)
         self.rt.tok[: self.M].copy_(tok.to(device=self.device, dtype=torch.int32))

@@ -33,9 +33,11 @@ class PagePool:
             raise ValueError(f"{pages} pages, at most {max_pages} per request, {max_tokens} tokens a call")
         if max(pages, max_pages) * page >= 2 ** 31:
             raise ValueError(f"{pages} pages, at most {max_pages} per request, of {page} tokens exceed 32-bit slots")
+        dev = torch.device(device)
+        if dev.type != "cuda":
+            raise ValueError(f"a page pool on {dev}: the serving operators have no CPU path")
         if not torch.cuda.is_available():
             raise RuntimeError("the page pool needs a CUDA device; there is no CPU path")
-        dev = torch.device(device)
         if dev.index is None:
             dev = torch.device("cuda", torch.cuda.current_device())
         self.requests, self.pages, self.max_pages, self.page, self.max_tokens, self.device = requests, pages, max_pages, page, max_tokens, dev
@@ -147,6 +149,7 @@ class Cache:
         at = lambda t: t.data_ptr() if t is not None else 0                            # noqa: E731
         self._args = (at(k), at(v), at(ks), at(vs), *strides, serve.INT4 if self.int4 else serve.TYPES[k.dtype], self.pages, self.kv_heads, self.head_dim, self.page, 0)
         self.desc = serve.CacheDesc(*self._args)
+        _status_of(self.device.index)
 
     def put(self, k, v, slots, stream=None):
         """Keys and values [tokens, kv heads, head dim] (fp32, bf16 or fp16) as they are to `slots` (int32 [tokens]); -1 is padding."""
@@ -243,16 +246,24 @@ _status, _bytes = {}, {}
 
 
 def _status_of(index):
-    """Where the calls on a device leave word of a wait that ran out."""
+    """Where the calls on a device leave word of a wait that ran out.  Its zeros are there before any stream's first call: not part of a graph, which would
+    write them at every replay."""
     st = _status.get(index)
     if st is None:
-        st = _status[index] = torch.zeros(4, dtype=torch.int32, device=index)
+        with torch.cuda.device(index):
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("the first paged.Cache of a device cannot be made inside a graph capture")
+            st = torch.zeros(4, dtype=torch.int32, device=index)
+            torch.cuda.current_stream().synchronize()
+        _status[index] = st
     return st
 
 
 def check(device=None):
     """Synchronise and raise if a device-side wait ran out in any call so far on this device (default: the current one)."""
-    index = torch.cuda.current_device() if device is None else torch.device(device).index
+    index = torch.device("cuda" if device is None else device).index
+    if index is None:
+        index = torch.cuda.current_device()
     st = _status_of(index).tolist()
     if st[0] != 0:
         _status_of(index).zero_()
@@ -268,7 +279,10 @@ def attend(q, cache, table, context, starts=None, max_new=None, scale=None, wind
     more than `max_new` (default: any number).  Query t of request r is at position context[r] - (starts[r + 1] - t) and sees the keys j up to its
     own position with j > position - window or j < sinks (window 0: all of them).  A query that sees nothing gives
     zeros; keys in a page that the table does not place inside the cache are not seen; rows of `out` outside the requests' queries are
-    left alone.  Query head h uses KV head h // (query heads / KV heads).  `scale` defaults to dim ** -0.5."""
+    left alone.  Query head h uses KV head h // (query heads / KV heads).  `scale` (positive) defaults to dim ** -0.5.
+
+    What no query of the call sees is not looked at and may hold anything.  Values that some query sees have to be finite: neighbouring queries
+    multiply the same tile of them, those that do not see a key by 0."""
     if not isinstance(cache, Cache):
         raise ValueError("cache: a paged.Cache")
     if q.dim() != 3 or q.dtype not in (torch.bfloat16, torch.float16) or (not cache.int4 and q.dtype != cache.dtype):
@@ -304,6 +318,8 @@ def attend(q, cache, table, context, starts=None, max_new=None, scale=None, wind
     (qt, qh, qd), (ot, oh, od) = q.stride(), out.stride()
     if qd != 1 or od != 1:
         raise ValueError("q, out: neighbouring dims")
+    if (T > 1 and ot < dim) or (nq > 1 and oh < dim):
+        raise ValueError(f"out: rows of {dim} overlap at strides {ot}, {oh}")
     fixed = (qt, qh, ot, oh, table.stride(0), *cache._args, 0, dim ** -0.5 if scale is None else scale, serve.TYPES[q.dtype], R, T, nq, pages, min(max_new, T),
              min(window, 2 ** 31 - 1), min(sinks, 2 ** 31 - 1), device)
     front = (q.data_ptr(), out.data_ptr(), table.data_ptr(), context.data_ptr(), starts.data_ptr() if starts is not None else 0)

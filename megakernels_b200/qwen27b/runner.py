@@ -207,7 +207,7 @@ class Engine(SequenceCalls):
         top_k, top_p, min_p; uniform numbers from `seed`), a launch or two per step."""
         if not self.lm_head:
             raise RuntimeError("generate needs the LM head")
-        if temperature > 0:
+        if self._sampled(temperature, top_k, top_p, min_p):
             if self.PK.tp > 1:
                 raise RuntimeError("sampling needs all logits on one GPU")
             return self._advance_sampled(tok, n_steps, temperature, top_k, top_p, min_p, seed)

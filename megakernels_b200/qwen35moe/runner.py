@@ -190,7 +190,7 @@ class Engine(SequenceCalls):
         (with a temperature: tokens sampled as `qwen27b.Engine.generate` does).  Returns the chosen ids [n_steps, M] (int32, on the device)."""
         if not self.lm_head:
             raise RuntimeError("generate needs the LM head")
-        if temperature > 0:
+        if self._sampled(temperature, top_k, top_p, min_p):
             return self._advance_sampled(tok, n_steps, temperature, top_k, top_p, min_p, seed)
         out = torch.zeros(n_steps, self.M, dtype=torch.int32, device=self.device)
         self.rt.tok[: self.M].copy_(tok.to(device=self.device, dtype=torch.int32))

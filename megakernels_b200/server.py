@@ -201,7 +201,7 @@ class Handler(BaseHTTPRequestHandler):
             if not isinstance(req.get("messages"), list):
                 raise KeyError("messages")
             filters_of(req)
-        except (ValueError, TypeError, KeyError) as e:
+        except (ValueError, TypeError, KeyError, OverflowError) as e:
             return self._reply(400, {"error": {"message": f"bad request: {e}"}})
         if not req.get("stream"):
             return self._reply(200, complete(self.session, req))

@@ -185,6 +185,12 @@ class SequenceCalls:
             _, live = self.pages.ask(self.pos[: self.M], part.shape[0])
             self.rt.launch(part.shape[0], tokens_out=part, row_valid=live)
 
+    def _sampled(self, temperature, top_k, top_p, min_p):
+        """Whether the tokens are sampled; refuses settings that mean nothing."""
+        from .. import sampling
+        sampling.check_settings(temperature, top_k, top_p, min_p)
+        return temperature > 0
+
     def _advance_sampled(self, tok, n_steps, temperature, top_k, top_p, min_p, seed):
         from .. import sampling
         return sampling.continue_from(lambda t: self.step(t), tok.to(self.device), n_steps, temperature, top_k, top_p, min_p, seed)

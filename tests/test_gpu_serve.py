@@ -321,6 +321,105 @@ def test_attend_leaves_other_rows_alone_and_takes_strides():
     assert bool((out[:, 1::2] == 5).all()) and bool((out[0] == 5).all()) and bool((out[6:] == 5).all())
 
 
+@pytest.mark.parametrize("kind,layout", [("bf16", "pages"), ("fp16", "serving"), ("int4", "pages")])
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 128), (256, 64)])
+def test_attend_many_queries_of_views(kind, layout, dim, page):
+    """Queries and outputs [heads, tokens, dim] and inside wider rows; a table inside a wider one; rows of out in front of and behind the queries."""
+    dtype = torch.float16 if kind == "fp16" else torch.bfloat16
+    cache, k, v, table, context, starts, q = case(kind, dtype, 6, 2, dim, page, [400, 130, 90], [150, 1, 90], 0, 0, seed=dim, layout=layout)
+    T = q.shape[0]
+    wide = torch.full((6, T + 9, dim + 8), 9.0, dtype=dtype, device=DEV)
+    wide[:, 5:T + 5, :dim] = q.transpose(0, 1)
+    out = torch.full((6, T + 9, dim + 64), 5.0, dtype=dtype, device=DEV)
+    big = torch.full((3, 70), -3, dtype=torch.int32, device=DEV)
+    big[:, 1: 1 + table.shape[1]] = table
+    for window, sinks in ((0, 0), (60, 9)):
+        got = paged.attend(wide[..., :dim].transpose(0, 1), cache, big[:, 1: 1 + table.shape[1]], context, starts=starts + 5, window=window, sinks=sinks, out=out[..., 64:].transpose(0, 1))
+        compare(got[5:T + 5], R.attend(q, k, v, table, context, starts, dim ** -0.5, window, sinks), cache, v, dtype, many=True)
+        assert bool((out[..., :64] == 5).all()) and bool((out[:, :5] == 5).all()) and bool((out[:, T + 5:] == 5).all())
+
+
+@pytest.mark.parametrize("kind", ["bf16", "int4"])
+@pytest.mark.parametrize("dim", [64, 256])
+def test_attend_many_queries_do_not_look_at_what_none_of_them_sees(kind, dim):
+    contexts, counts, window, sinks = [600, 257, 0, 40], [190, 100, 70, 40], 20, 2
+    cache, k, v, table, context, starts, q = case(kind, torch.bfloat16, 4, 2, dim, 16, contexts, counts, window, sinks, seed=19)
+    table[0, 30], table[3, 0] = 10 ** 6, -7                     # keys 480 .. 495 of request 0, 0 .. 15 of request 3
+    seen = torch.zeros(cache.pages, cache.page, dtype=torch.bool, device=DEV)
+    for r, (c, n) in enumerate(zip(contexts, counts)):
+        for j in range(c):
+            page = int(table[r, j // 16])
+            if (j < sinks or j > c - n - window) and 0 <= page < cache.pages:
+                seen[page, j % 16] = True
+    for t in (cache.k_scales, cache.v_scales) if kind == "int4" else (cache.k, cache.v):
+        t.copy_(torch.where(seen[:, None, :].reshape(cache.pages, 1, cache.page, *([1] * (t.dim() - 3))), t, math.nan))
+    got = paged.attend(q, cache, table, context, starts=starts, window=window, sinks=sinks)
+    want = R.attend(q, torch.nan_to_num(k), torch.nan_to_num(v), table, context, starts, dim ** -0.5, window, sinks)
+    near(got, want, HALF[torch.bfloat16], (2.0 ** -8 if kind == "bf16" else 3 * 2.0 ** -11 + 2.0 ** -14) * float(torch.nan_to_num(v).abs().max()) * (1 if kind == "bf16" else 2.2))
+    assert bool((got[290:360] == 0).all())                      # the request without positions
+    paged.check()
+
+
+def test_attend_many_queries_in_graphs_and_on_streams_at_once():
+    cache, k, v, table, context, starts, q = case("bf16", torch.bfloat16, 8, 2, 256, 64, [900, 600], [500, 400], 0, 0, seed=8)
+    want = paged.attend(q, cache, table, context, starts=starts)
+    outs, graphs = [], []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(paged.attend(q, cache, table, context, starts=starts))
+        graphs.append(graph)
+    q.mul_(0.5)
+    half = paged.attend(q, cache, table, context, starts=starts)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for s, graph in zip(streams, graphs):
+        with torch.cuda.stream(s):
+            graph.replay()
+    few = paged.attend(q[:2], cache, table, context, stream=streams[2])
+    also = paged.attend(q, cache, table, context, starts=starts, stream=streams[2])
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], half) and torch.equal(outs[1], half) and torch.equal(also, half) and not torch.equal(want, half)
+    assert torch.equal(few, paged.attend(q[:2], cache, table, context))
+    paged.check("cuda")
+
+
+def test_attend_takes_more_queries_than_it_was_told_of():
+    """max_new chooses a kernel and bounds nothing."""
+    cache, k, v, table, context, starts, q = case("bf16", torch.bfloat16, 4, 2, 64, 16, [90, 70], [33, 12], 0, 0, seed=4)
+    got = paged.attend(q, cache, table, context, starts=starts, max_new=1)
+    compare(got, R.attend(q, k, v, table, context, starts, 0.125), cache, v, torch.bfloat16, many=True)
+
+
+@pytest.mark.parametrize("kind,dim,new", [("bf16", 256, 1), ("int4", 64, 9)])
+def test_attend_of_the_most_requests(kind, dim, new):
+    R_, T = 4096, 4096 * new
+    cache = make_cache(kind, 65, 4, dim, 16)
+    k, v = fill(cache, 2)
+    table = (torch.arange(R_, dtype=torch.int32, device=DEV) % 64 + 1).view(R_, 1)
+    context = torch.full((R_,), 16, dtype=torch.int32, device=DEV)
+    starts = torch.arange(R_ + 1, dtype=torch.int32, device=DEV) * new
+    q = torch.randn(64 * new, 16, dim, generator=gen(3), device=DEV).to(torch.bfloat16)
+    got = paged.attend(q.repeat(64, 1, 1), cache, table, context, starts=starts, max_new=new)
+    want = R.attend(q, k, v, table[:64], context[:64], starts[:65], dim ** -0.5)
+    assert got.shape[0] == T and torch.equal(got.view(64, -1), got[: 64 * new].reshape(1, -1).expand(64, -1))
+    compare(got[: 64 * new], want, cache, v, torch.bfloat16, many=True)
+
+
+@pytest.mark.parametrize("kind,layout", [("bf16", "serving"), ("fp16", "pages")])
+@pytest.mark.parametrize("source", [torch.float32, torch.bfloat16, torch.float16])
+def test_put_writes_rows_as_they_are(kind, layout, source):
+    cache = make_cache(kind, 4, 2, 64, 16, layout)
+    k, v = (torch.randn(5, 2, 64, generator=gen(i), device=DEV).to(source) for i in range(2))
+    slots = ints([17, -1, 63, 16, 64])
+    cache.put(k, v, slots)
+    got_k, got_v = cache.rows(slots)
+    for got, x in ((got_k, k), (got_v, v)):
+        assert torch.equal(got[[0, 2, 3]], x[[0, 2, 3]].to(cache.dtype)) and bool((got[[1, 4]] == 0).all())
+    assert int((cache.k != 0).any(-1).sum()) == 6               # three rows of two heads
+
+
 @pytest.mark.parametrize("spread", [1e-6, 1.0, 3e4])
 @pytest.mark.parametrize("dtype", [torch.bfloat16])
 def test_attend_values_of_any_size(spread, dtype):

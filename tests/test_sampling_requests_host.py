@@ -88,6 +88,22 @@ def test_a_request_that_means_nothing_is_refused(session):
         httpd.shutdown()
 
 
+def test_a_request_with_numbers_beyond_all_bounds_is_refused(session):
+    """JSON as Python reads it has Infinity and NaN."""
+    httpd = server.serve(session, port=0)
+    threading.Thread(target=httpd.serve_forever, daemon=True).start()
+    try:
+        url = f"http://127.0.0.1:{httpd.server_address[1]}/v1/chat/completions"
+        for bad in ('"top_k": Infinity', '"top_p": NaN', '"min_p": -Infinity', '"top_k": 1e400'):
+            body = '{"messages": [{"role": "user", "content": "hi"}], %s}' % bad
+            with pytest.raises(urllib.error.HTTPError) as e:
+                urllib.request.urlopen(urllib.request.Request(url, body.encode()), timeout=20)
+            assert e.value.code == 400
+        assert not session.mk.asked
+    finally:
+        httpd.shutdown()
+
+
 def test_the_chat_loop_passes_them_on(session):
     lines = iter(["hello", "/quit"])
     repl(session, inp=lambda _: next(lines), out=io.StringIO(), top_k=7, top_p=0.8, min_p=0.0)

@@ -175,6 +175,31 @@ def test_python_refusals_come_before_the_gpu():
         paged.attend(q.bfloat16(), None, at, at)
 
 
+def test_refusals_of_scales_and_of_rows_that_overlap(lib_built):
+    lib = serve.lib()
+    good = dict(q=4096, out=4096, table=4096, context=4096, starts=0, workspace=4096, status=4096, q_tok=512, q_head=128, out_tok=512, out_head=128, table_stride=8, cache=cache(), spin_limit_ns=0,
+                scale=0.1, type=serve.BF16, requests=3, tokens=3, q_heads=4, max_pages=8, max_new=1, window=0, sinks=0, device=0)
+    for scale in (0.0, -0.5, float("nan"), float("inf"), 2e30):
+        refused(lib, lib.mk_attend(bytes(serve.AttendArgs(**dict(good, scale=scale))), None))
+        refused(lib, lib.mk_attend_bytes(bytes(serve.AttendArgs(**dict(good, scale=scale)))))
+    for bad in (dict(out_tok=0), dict(out_tok=64), dict(out_head=0), dict(out_head=120)):
+        refused(lib, lib.mk_attend(bytes(serve.AttendArgs(**dict(good, **bad))), None))
+
+
+def test_a_pool_belongs_on_a_gpu():
+    with pytest.raises(ValueError, match="no CPU path"):
+        paged.PagePool(4, 10, 4, device="cpu")
+
+
+def test_engines_refuse_settings_that_mean_nothing():
+    from megakernels_b200.stage.kv import SequenceCalls
+    eng = SequenceCalls()
+    assert eng._sampled(0.5, 10, 0.9, 0.0) and not eng._sampled(0.0, 0, 1.0, 0.0)
+    for bad in ((-0.5, 0, 1.0, 0.0), (float("nan"), 0, 1.0, 0.0), (0.0, -1, 1.0, 0.0), (1.0, 0, 0.0, 0.0), (1.0, 0, 1.0, 2.0)):
+        with pytest.raises(ValueError):
+            eng._sampled(*bad)
+
+
 # ---- what the other tests compare with ---------------------------------------------------------------------------
 def test_the_reference_attention_is_a_softmax():
     g = torch.Generator().manual_seed(0)
