@@ -1,6 +1,6 @@
 // Attention over a paged cache (declarations and rule: include/mk_serve.h).
 //
-// attend_step: few queries per request.  Rows are the (token, query head) pairs of a KV head, eight at a time; a unit is (request, KV
+// attend_step: few rows per SM (by_tiles).  Rows are the (token, query head) pairs of a KV head, eight at a time; a unit is (request, KV
 // head, eight rows), and its work the tiles of 16 keys that they see.  All tiles of a call form one line, dealt to the CTAs in equal
 // runs; inside a run a warp takes every eighth (sixth, twelfth) tile, on its own: it copies the tile's rows into a ring of its own (cp.async, no barrier),
 // multiplies them as they lie and keeps running maxima, sums and outputs in registers.  Scores are keys x dims x queries with
@@ -506,7 +506,7 @@ static __global__ void __launch_bounds__(Layout<HD, KIND>::WARPS * 32, 1) attend
 
 // Block (c, y) adds up 64 dims of the unit that starts in CTA c and does not end there: its part, then one part of every following CTA until the one that
 // ends it.  Maxima and sums of all parts first, side by side, so that nothing is carried from part to part: a single long context is in as many parts
-// as there are CTAs (30000 positions of one request, one part after the other: 93 us a call; so 25).
+// as there are CTAs (30000 positions of one request, one part after the other: 93 us a call; so 21).
 constexpr int J_GROUPS = 4, J_THREADS = J_GROUPS * 256, J_PARTS = 256;
 template <int HD>
 static __global__ void __launch_bounds__(J_THREADS) attend_join(const __grid_constant__ AttendArgs A, int ctas) {
@@ -585,6 +585,22 @@ static int launch_kind(const AttendArgs& A, int type, int sms, cudaStream_t st) 
     return type == MKV_INT4 ? launch_step<HD, K_INT4>(A, sms, st) : (type == MKV_F16 ? launch_step<HD, K_F16>(A, sms, st) : launch_step<HD, K_BF16>(A, sms, st));
 }
 
+// Which kernel: attend_step reads a request's keys once per eight rows, evenly over all SMs; attend_rows once per 256 (heads of 64: 128), but a pair of
+// SMs (an SM) takes all keys of its rows, so the call lasts as many passes as pairs have blocks.  A unit of eight rows costs an SM about what a pass costs a pair: the step
+// where there are no more units per SM than passes.  Requests may differ: counted from max_new, or as if half of the last unit (block) of each were empty.  Us, step and tiles, 16 requests of 4000 positions: 16 / 2 heads of 256, bf16, 8, 32, 64 rows
+// 39 67, 68 68, 122 68; 24 / 4 heads, 12, 30 rows 68 70, 171 71 (4 bits 68 116, 116 116); 32 / 8 heads of 128, 16, 32 rows 92 104, 166 104 (4 bits 80 151, 146 149);
+// 8 / 8 heads of 64, 8, 16 rows 36 54, 56 54.  One request of 8000, 16 / 2 heads of 256: 64, 128 rows 30 112, 41 114.
+static bool by_tiles(const AttendArgs& A, int max_new, int head_dim, int sms) {
+    const int cg = head_dim >= 128 ? 2 : 1;
+    auto count = [&](long long rows) {
+        const long long busy = A.R < A.T ? A.R : A.T, each = busy * (((long long)max_new * A.per + rows - 1) / rows), half = (long long)A.T * A.per / rows + busy / 2;
+        const long long all = half > busy ? half : busy;
+        return A.nkv * (each < all ? each : all);
+    };
+    const long long passes = (count(128 * cg) + sms / cg - 1) / (sms / cg);
+    return count(8) > passes * sms;
+}
+
 static const char* bad_attend(const mk_attend_args* a) {
     if (const char* why = bad_cache(a->cache)) return why;
     const mk_cache& c = a->cache;
@@ -648,6 +664,6 @@ extern "C" int mk_attend(const mk_attend_args* a, void* stream) {
     A.spin_limit_ns = a->spin_limit_ns > 0 ? a->spin_limit_ns : 2000000000ll;
     A.scale_log2 = a->scale * 1.4426950408889634f;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if ((int64_t)a->max_new * A.per > 32) return launch_rows(A, c.type, c.head_dim, sms, st);
+    if (by_tiles(A, a->max_new, c.head_dim, sms)) return launch_rows(A, c.type, c.head_dim, sms, st);
     return c.head_dim == 64 ? launch_kind<64>(A, c.type, sms, st) : (c.head_dim == 128 ? launch_kind<128>(A, c.type, sms, st) : launch_kind<256>(A, c.type, sms, st));
 }

@@ -385,6 +385,28 @@ def test_attend_many_queries_in_graphs_and_on_streams_at_once():
     paged.check("cuda")
 
 
+@pytest.mark.parametrize("kind,dim", [("bf16", 64), ("bf16", 256), ("int4", 128)])
+def test_attend_sharp_scores_of_many_queries(kind, dim):
+    """Scores that rise far above what came before, tile after tile: what was added is scaled away each time."""
+    cache, k, v, table, context, starts, q = case(kind, torch.bfloat16, 4, 2, dim, 64, [1500, 700], [900, 650], 0, 0, seed=16)
+    q.mul_(20)
+    got = paged.attend(q, cache, table, context, starts=starts)
+    want = R.attend(q, k, v, table, context, starts, dim ** -0.5)
+    # scores reach 20 * 2 * |k|'s 4 sigma over dim ** -0.5 sums: below 20 * 2 * 4 * 16; their 32-bit error, 2^-20 of that, is the exponent's, on either side of a quotient
+    near(got, want, HALF[torch.bfloat16], (2.0 ** -8 + 3 * 2.0 ** -11 + 2 * 2.0 ** -20 * 2560) * 2 * float(v.abs().max()))
+    paged.check()
+
+
+@pytest.mark.parametrize("spread", [1e-6, 1.0, 3e4])
+def test_attend_many_queries_on_values_of_any_size(spread):
+    """4-bit values far below and above what a half can hold."""
+    cache, k, v, table, context, starts, q = case("int4", torch.bfloat16, 4, 1, 128, 16, [900, 440], [700, 440], 0, 0, seed=15, spread=spread)
+    cache.k_scales.copy_(cache.k_scales * (1 / spread))
+    k = R.decode(cache.k, cache.k_scales)
+    got = paged.attend(q, cache, table, context, starts=starts)
+    compare(got, R.attend(q, k, v, table, context, starts, 128 ** -0.5), cache, v, torch.bfloat16, many=True)
+
+
 def test_attend_takes_more_queries_than_it_was_told_of():
     """max_new chooses a kernel and bounds nothing."""
     cache, k, v, table, context, starts, q = case("bf16", torch.bfloat16, 4, 2, 64, 16, [90, 70], [33, 12], 0, 0, seed=4)
