@@ -7,7 +7,7 @@
 //   S = Q K^T    Q and K from shared memory (both K-major), 128 scores a row into one of two accumulators in tensor memory;
 //   O += P V     P from tensor memory, where the row's threads put it over its scores, V from shared memory as it lies (MN-major).
 // Each CTA of a pair brings half of a tile: 64 of its keys, and half of the dims of all its values.  So a 4-bit tile is turned into halves once per 256 rows
-// (two prompts of 1500 of 4000 positions, 24 / 4 heads of 256: 423 us alone, 283 in pairs), and the L2 is read half as often.
+// (two prompts of 1500 of 4000 positions, 24 / 4 heads of 256: 423 us alone, 283 in pairs), and a prompt of 8192 moves 1.08 GB through the L2, not 1.31.
 //   While the softmax works on tile i, the products of S(i + 1) and P(i - 1) V run.  Two threads of a row exchange its maximum over a barrier of their two
 // warps: a barrier of all eight, or a whole row per thread with the warps by turns over the tiles, both take longer (prompt of 8192: 216 and 226 us, 198 so).
 // Outputs are scaled again only when a row's maximum rises by 2^8 (in tensor memory, by the row's threads, behind the product before).
